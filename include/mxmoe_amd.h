@@ -300,6 +300,69 @@ int mxmoe_combine_sorted(const void* down_out, const int64_t* recv_tokens_per_ex
  * a few KB): the host array may be changed or freed as soon as the call returns, and the call waits for nothing. */
 int mxmoe_upload(void* dst, const void* host_src, size_t bytes, void* stream);
 
+/* ---- tokens sorted by expert and back, in any float type, with gradients (no counterpart in the reference, which sorts with torch::sort +
+ *      index_select, mxmoe/kernels/src/ref_bind.cu:47-64, and leaves the way back an empty stub, :66) ----
+ *
+ * dtype: 0 fp16, 1 fp32, 2 bf16.  Rows hold K elements; `ld*` is the distance of two rows of an input in elements (>= 0: 0 repeats one row), outputs are
+ * packed.  No pointer needs more alignment than its element.  1 <= topk <= 64, experts <= 4096, num_tokens * topk <= 2^30, error 3 otherwise;
+ * num_tokens = 0 is allowed.  num_rows: rows that `rows` / `grad_rows` hold; a map that names others names nothing.
+ *
+ * mxmoe_permute_tokens   row(t, s), the place of slot s of token t, in stable order by (expert, t * topk + s); ids outside [0, E) come last.  Writes
+ *     rows[row(t, s)] = hidden[t], zeros for ids out of range (keep_tail != 0: those rows, which lie behind the last routed one, are left as they were);
+ *     row_of_slot[t * topk + s] = row(t, s), or -2 - row(t, s) for an id out of range; recv_tokens_per_exp [E]; and perm_indices [num_tokens * topk]
+ *     (may be NULL), the token behind each routed row.  topk_ids int32 or int64 (ids_bytes 4 or 8).  rows must not overlap hidden.
+ *     workspace: mxmoe_permute_tokens_workspace_bytes bytes (none: may be NULL), 16-byte aligned.
+ * mxmoe_unpermute_tokens out[t] = sum_s topk_weights[t, s] * rows[row(t, s)] + shared[t], fp32, products and sums rounded one by one in slot order, one
+ *     rounding to dtype (fp16: the bits of mxmoe_combine_sorted).  Negative entries of row_of_slot contribute nothing.  topk_weights NULL: all 1 (the
+ *     gradient of mxmoe_permute_tokens is this call on the rows' gradients); shared NULL: none.
+ * mxmoe_unpermute_tokens_backward   grad_rows[row(t, s)] = topk_weights[t, s] * grad_out[t], and zeros (keep_tail != 0: nothing) in the row that a
+ *     dropped slot's entry -2 - row names (an entry -1 names none); grad_weights[t, s] = <grad_out[t], rows[row(t, s)]> in fp32, 0 for a dropped slot.
+ *     topk_weights NULL: all 1; grad_weights NULL: not wanted, and rows
+ *     is not read.  grad_shared is grad_out. */
+size_t mxmoe_permute_tokens_workspace_bytes(int num_tokens, int topk, int num_experts);
+int mxmoe_permute_tokens(const void* hidden, int64_t ld, int dtype, const void* topk_ids, int ids_bytes, int num_tokens, int topk, int num_experts, int K, void* rows, int keep_tail,
+                         int32_t* row_of_slot, int64_t* recv_tokens_per_exp, int64_t* perm_indices, void* workspace, void* stream);
+int mxmoe_unpermute_tokens(const void* rows, int64_t ld, int num_rows, const int32_t* row_of_slot, const float* topk_weights, const void* shared, int64_t ld_shared, int dtype,
+                           int num_tokens, int topk, int K, void* out, void* stream);
+int mxmoe_unpermute_tokens_backward(const void* grad_out, int64_t ld_grad, const void* rows, int64_t ld, int num_rows, const int32_t* row_of_slot, const float* topk_weights, int dtype,
+                                    int num_tokens, int topk, int K, void* grad_rows, int keep_tail, float* grad_weights, void* stream);
+
+/* Gradient of mxmoe_route_topk (mxmoe/quant/moe_tracer.py:79-86 is differentiated by autograd there): grad_weights [num_tokens, topk] fp32 -> grad_logits
+ * [num_tokens, num_experts] in the logits' type, for the chosen topk_ids.  p = softmax of the logits in fp32 (renormalise: of the chosen ones);
+ * inner = sum_s grad_weights[s] * p[topk_ids[s]]; grad_logits[j] = p[j] * (sum of grad_weights of the slots that chose j - inner), with renormalise
+ * p[j] * (sum over the slots that chose j of grad_weights - inner), 0 for experts that were not chosen.  Ids out of range take no part.  Limits as mxmoe_route_topk. */
+int mxmoe_route_topk_backward(const float* grad_weights, const void* router_logits, int logits_dtype, const int32_t* topk_ids, int num_tokens, int num_experts, int topk, int renormalise,
+                              void* grad_logits, void* stream);
+
+/* ---- the norms before and after a block, its gate and its residual scale, with gradients (no counterpart in the reference, whose kernels end at the
+ *      block's own linear layers) ----
+ *
+ * x and h: the residual stream, x_dtype; z and y: the block's output and the next block's input, z_dtype (y_dtype); any two of fp16 (0), fp32 (1), bf16 (2).
+ * norm_weight (w1), next_weight (w2), scale: [K] in weight_dtype, each may be NULL.  1 <= K <= 32768; `ld*` and alignment as above; num_tokens = 0 is allowed.
+ *
+ * mxmoe_block_norm       y = x / sqrt(mean x^2 + eps) * weight                              (weight NULL: 1)
+ * mxmoe_block_residual   n = z / sqrt(mean z^2 + eps) * w1                                  (w1 NULL: n = z)
+ *                        a = gate, or 1 / (1 + exp(-gate)) with sigmoid                     (gate_kind 0: 1; 1: gate[t * ld_gate] of gate_dtype; 2: gate
+ *                                                                                            rows of K of z's type)
+ *                        h = x + factor * scale * a * n                                     (scale NULL: 1)
+ *                        y = h / sqrt(mean h^2 + eps) * w2                                  (y NULL: not wanted; w2 NULL: 1)
+ *     All in fp32; h and y are rounded once, y comes from the unrounded h.  h may be x itself (same rows, ldx = K), so may y be z; no other overlap.
+ * mxmoe_block_*_backward   the gradients of all inputs, sums over the tokens in fp32 and in a fixed order.  grad_y may be NULL (y was not used) and so may
+ *     grad_h (grad_residual: what reaches x on other ways and is added to its gradient), not both.  grad_gate: gate_kind 1 packed [num_tokens] of gate_dtype,
+ *     2 [num_tokens, K].  Gradients of the vectors that are given are written, in weight_dtype, also for no tokens (zeros).
+ *     workspace: mxmoe_block_backward_workspace_bytes bytes, 16-byte aligned; NULL where no vector is given. */
+int mxmoe_block_norm(const void* x, int64_t ldx, int x_dtype, const void* weight, int weight_dtype, float eps, int num_tokens, int K, void* y, int y_dtype, void* stream);
+int mxmoe_block_residual(const void* x, int64_t ldx, int x_dtype, const void* z, int64_t ldz, int z_dtype, int gate_kind, const void* gate, int64_t ld_gate, int gate_dtype, int sigmoid,
+                         float factor, const void* scale, const void* norm_weight, const void* next_weight, int weight_dtype, float eps, int num_tokens, int K, void* h, void* y,
+                         void* stream);
+size_t mxmoe_block_backward_workspace_bytes(int num_tokens, int K);
+int mxmoe_block_norm_backward(const void* grad_y, int64_t ld_grad_y, int y_dtype, const void* x, int64_t ldx, int x_dtype, const void* weight, int weight_dtype, const void* grad_residual,
+                              int64_t ld_grad_residual, float eps, int num_tokens, int K, void* grad_x, void* grad_weight, void* workspace, void* stream);
+int mxmoe_block_residual_backward(const void* grad_h, int64_t ld_grad_h, const void* grad_y, int64_t ld_grad_y, const void* x, int64_t ldx, int x_dtype, const void* z, int64_t ldz,
+                                  int z_dtype, int gate_kind, const void* gate, int64_t ld_gate, int gate_dtype, int sigmoid, float factor, const void* scale, const void* norm_weight,
+                                  const void* next_weight, int weight_dtype, float eps, int num_tokens, int K, void* grad_x, void* grad_z, void* grad_gate, void* grad_scale,
+                                  void* grad_norm_weight, void* grad_next_weight, void* workspace, void* stream);
+
 /* ---- the planned forward in its short form ----
  *
  * One call enqueues the whole forward of one layer for one (tokens, top-k): permutation, planning and the quantisation of every

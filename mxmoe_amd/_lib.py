@@ -38,6 +38,8 @@ class QParams(C.Structure):
 
 _P = C.c_void_p
 _I = C.c_int
+_L = C.c_int64
+_F = C.c_float
 
 # name -> (restype, argtypes); mirrors include/mxmoe_amd.h declaration by declaration
 SIGNATURES = {
@@ -91,6 +93,16 @@ SIGNATURES = {
     "mxmoe_layer_create": (_I, [_P, C.POINTER(_P)]),
     "mxmoe_layer_destroy": (None, [_P]),
     "mxmoe_layer_run": (_I, [_P, _P, _P, _P, _P, _P]),
+    "mxmoe_permute_tokens_workspace_bytes": (C.c_size_t, [_I, _I, _I]),
+    "mxmoe_permute_tokens": (_I, [_P, _L, _I, _P, _I, _I, _I, _I, _I, _P, _I, _P, _P, _P, _P, _P]),
+    "mxmoe_unpermute_tokens": (_I, [_P, _L, _I, _P, _P, _P, _L, _I, _I, _I, _I, _P, _P]),
+    "mxmoe_unpermute_tokens_backward": (_I, [_P, _L, _P, _L, _I, _P, _P, _I, _I, _I, _I, _P, _I, _P, _P]),
+    "mxmoe_route_topk_backward": (_I, [_P, _P, _I, _P, _I, _I, _I, _I, _P, _P]),
+    "mxmoe_block_norm": (_I, [_P, _L, _I, _P, _I, _F, _I, _I, _P, _I, _P]),
+    "mxmoe_block_residual": (_I, [_P, _L, _I, _P, _L, _I, _I, _P, _L, _I, _I, _F, _P, _P, _P, _I, _F, _I, _I, _P, _P, _P]),
+    "mxmoe_block_backward_workspace_bytes": (C.c_size_t, [_I, _I]),
+    "mxmoe_block_norm_backward": (_I, [_P, _L, _I, _P, _L, _I, _P, _I, _P, _L, _F, _I, _I, _P, _P, _P, _P]),
+    "mxmoe_block_residual_backward": (_I, [_P, _L, _P, _L, _P, _L, _I, _P, _L, _I, _I, _P, _L, _I, _I, _F, _P, _P, _P, _I, _F, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P]),
     "mxmoe_combine_workspace_bytes": (C.c_size_t, [_I, _I]),
     "mxmoe_unpermute_combine": (_I, [_P, _P, _P, _P, _I, _I, _I, _I, _P, _P, _P]),
 }

@@ -1,0 +1,411 @@
+"""The operators of one MoE block around its experts' products, forward and backward:
+
+  permute_tokens     tokens sorted by expert           } with the experts' products of `ops.gg_*` or of the caller between them
+  unpermute_tokens   and back, weighted                }
+  block_norm         the norm in front of a block
+  block_residual     a block's output normed, gated and scaled onto the residual stream, and the next block's norm of the sum
+  route_topk_backward, *_backward   the gradients, as calls of their own
+
+They run the kernels of `include/mxmoe_amd.h` of the same names (the reference has no counterpart of most: its permutation is torch::sort + index_select,
+mxmoe/kernels/src/ref_bind.cu:47-64, its way back an empty stub, :66) on fp16, bf16 and fp32 rows, with sums in fp32.  All of them enqueue kernels on the current
+stream of their tensors' device, wait for nothing and can be captured into a HIP graph.  They are exported by `mxmoe_amd.ops`.
+
+Where an input requires a gradient (and gradients are enabled) the forward operators record themselves for autograd.  That form is refused while a stream is being
+captured (autograd synchronises with the streams of the leaves' earlier graphs, which a capture does not survive): a captured training step calls the `*_backward`
+operators.
+"""
+from __future__ import annotations
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+
+_TYPES = {torch.float16: 0, torch.float32: 1, torch.bfloat16: 2}
+_NO_TYPE = "{} of dtype {}: fp16, fp32 or bf16 expected"
+
+
+def _call(dev: torch.device, name: str, *args) -> None:
+    """Entry point `name` on the current stream of `dev` (the library launches on the current device, whose stream it must be)."""
+    lib = _lib.load()
+    if dev.index == torch.cuda.current_device():
+        rc = getattr(lib, name)(*args, _lib.current_stream())
+    else:
+        with torch.cuda.device(dev):
+            rc = getattr(lib, name)(*args, _lib.current_stream())
+    if rc:
+        _lib.check(lib, rc)
+
+
+def _rows(x: torch.Tensor, name: str, shape=None, dtype=None, dev=None) -> torch.Tensor:
+    """x as rows the kernels can read: 2-D, elements side by side (any row stride), a float type, on the GPU."""
+    if x.dim() != 2 or (shape is not None and tuple(x.shape) != shape):
+        raise ValueError(f"{name} of shape {list(x.shape)}: " + ("rows expected, [tokens, K]" if shape is None else f"{list(shape)} expected"))
+    if x.dtype not in _TYPES or (dtype is not None and x.dtype != dtype):
+        raise ValueError(_NO_TYPE.format(name, x.dtype) if dtype is None else f"{name} of dtype {x.dtype}: {dtype} expected")
+    _on(x, name, dev)
+    return x if x.stride(1) == 1 or x.shape[1] == 1 else x.contiguous()
+
+
+def _on(x: torch.Tensor, name: str, dev) -> None:
+    if not x.is_cuda or (dev is not None and x.device != dev):
+        raise ValueError(f"{name} is on {x.device}: " + (f"{dev} expected" if dev is not None else "a GPU expected"))
+
+
+def _output(out, shape, dtype, dev) -> torch.Tensor:
+    if out is None:
+        return torch.empty(shape, dtype=dtype, device=dev)
+    if tuple(out.shape) != tuple(shape) or out.dtype != dtype or out.device != dev or not out.is_contiguous():
+        raise ValueError(f"out: a contiguous tensor of shape {list(shape)} and dtype {dtype} on {dev} expected")
+    return out
+
+
+def _recorded(*tensors, out=None) -> bool:
+    """Whether autograd is to record a call with these inputs."""
+    if not torch.is_grad_enabled() or not any(isinstance(t, torch.Tensor) and t.requires_grad for t in tensors):
+        return False
+    if out is not None:
+        raise ValueError("out= is for calls without gradients")
+    if torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("gradients are not recorded while a stream is being captured: call the operator under torch.no_grad() and its *_backward in the captured step")
+    return True
+
+
+# ---- tokens sorted by expert ----
+
+def permute_tokens(hidden: torch.Tensor, topk_ids: torch.Tensor, num_experts: int, out: torch.Tensor | None = None):
+    """Tokens [T, K] sorted by the experts they go to -> (rows [T * k, K], row_of_slot int32 [T, k], recv_tokens_per_exp int64 [E] on the device).
+
+    Stable order by (expert, flattened (token, slot)), as `build_permutation`.  Ids (int32 or int64) outside [0, E), such as -1 for padding tokens or for experts of
+    another GPU, name no expert: their rows come behind all others and are zero, and row_of_slot holds -2 - row for them.  With `out` [T * k, K] the rows go there,
+    and those behind the last routed one are left as they were."""
+    if _recorded(hidden, out=out):
+        return _Permute.apply(hidden, topk_ids, num_experts, None)
+    return _permute(hidden, topk_ids, num_experts, out, None)
+
+
+def _permute(hidden, topk_ids, num_experts, out, perm):
+    x = _rows(hidden, "hidden")
+    t, k = x.shape
+    dev = x.device
+    if topk_ids.dim() != 2 or topk_ids.shape[0] != t:
+        raise ValueError(f"topk_ids of shape {list(topk_ids.shape)}: [{t}, top-k] expected")
+    if topk_ids.dtype != torch.int32 and topk_ids.dtype != torch.int64:
+        raise ValueError(f"topk_ids of dtype {topk_ids.dtype}: int32 or int64 expected")
+    _on(topk_ids, "topk_ids", dev)
+    ids = topk_ids.contiguous()
+    topk = ids.shape[1]
+    rows = _output(out, (t * topk, k), x.dtype, dev)
+    row_of_slot = torch.empty((t, topk), dtype=torch.int32, device=dev)
+    recv = torch.empty(max(num_experts, 0), dtype=torch.int64, device=dev)
+    need = _lib.load().mxmoe_permute_tokens_workspace_bytes(t, topk, num_experts)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    _call(dev, "mxmoe_permute_tokens", x.data_ptr(), x.stride(0), _TYPES[x.dtype], ids.data_ptr(), ids.element_size(), t, topk, num_experts, k, rows.data_ptr(), out is not None,
+          row_of_slot.data_ptr(), recv.data_ptr(), None if perm is None else perm.data_ptr(), None if ws is None else ws.data_ptr())
+    return rows, row_of_slot, recv
+
+
+def permute_with_indices(hidden, topk_ids, num_experts, perm):
+    """(rows, counts on the host) of `permute_tokens`, and the token behind each routed row in `perm` int64 [T * k] (what `gg_permute_inp` returns)."""
+    if _recorded(hidden):
+        rows, _m, recv = _Permute.apply(hidden, topk_ids, num_experts, perm)
+    else:
+        rows, _m, recv = _permute(hidden, topk_ids, num_experts, None, perm)
+    return rows, recv.cpu()
+
+
+def permute_tokens_backward(grad_rows: torch.Tensor, row_of_slot: torch.Tensor) -> torch.Tensor:
+    """Gradient of `permute_tokens`: grad_hidden[t] = sum of the gradients of token t's rows (fp32, in slot order, rounded once)."""
+    return unpermute_tokens(grad_rows.detach(), row_of_slot)
+
+
+def _map(row_of_slot, dev):
+    if row_of_slot.dim() != 2 or row_of_slot.dtype != torch.int32:
+        raise ValueError(f"row_of_slot: int32 [tokens, top-k] expected, got {row_of_slot.dtype} {list(row_of_slot.shape)}")
+    _on(row_of_slot, "row_of_slot", dev)
+    return row_of_slot.contiguous()
+
+
+def _weights(topk_weights, m, dev):
+    if topk_weights is None:
+        return None
+    if topk_weights.shape != m.shape:
+        raise ValueError(f"topk_weights of shape {list(topk_weights.shape)}: {list(m.shape)} expected")
+    _on(topk_weights, "topk_weights", dev)
+    return topk_weights.to(torch.float32).contiguous()
+
+
+def unpermute_tokens(rows: torch.Tensor, row_of_slot: torch.Tensor, topk_weights: torch.Tensor | None = None, shared: torch.Tensor | None = None,
+                     out: torch.Tensor | None = None) -> torch.Tensor:
+    """Sorted rows back in token order: out[t] = sum_s topk_weights[t, s] * rows[row_of_slot[t, s]] (+ shared[t]), slots with a negative entry left out; fp32 in slot
+    order, rounded once (for fp16 the bits of `gg_unpermute_out`).  A token none of whose slots names a row gets zeros (or its shared row).  Without weights all are 1."""
+    if _recorded(rows, topk_weights, shared, out=out):
+        return _Unpermute.apply(rows, row_of_slot, topk_weights, shared)
+    x = _rows(rows, "rows")
+    dev, k = x.device, x.shape[1]
+    m = _map(row_of_slot, dev)
+    w = _weights(topk_weights, m, dev)
+    t, topk = m.shape
+    sh = None if shared is None else _rows(shared, "shared", (t, k), x.dtype, dev)
+    y = _output(out, (t, k), x.dtype, dev)
+    _call(dev, "mxmoe_unpermute_tokens", x.data_ptr(), x.stride(0), x.shape[0], m.data_ptr(), None if w is None else w.data_ptr(), None if sh is None else sh.data_ptr(),
+          0 if sh is None else sh.stride(0), _TYPES[x.dtype], t, topk, k, y.data_ptr())
+    return y
+
+
+def unpermute_tokens_backward(grad_out: torch.Tensor, rows: torch.Tensor | None, row_of_slot: torch.Tensor, topk_weights: torch.Tensor | None = None,
+                              num_rows: int | None = None, out: torch.Tensor | None = None):
+    """Gradients of `unpermute_tokens` -> (grad_rows [rows, K], grad_weights fp32 [T, k]); that of `shared` is grad_out itself.
+
+    grad_rows[row_of_slot[t, s]] = w[t, s] * grad_out[t]; rows that belong to dropped slots (those behind the last routed one, as `permute_tokens` numbers them) are zero,
+    with `out` left as they were.  `rows` None (then `num_rows`, default T * k, says how many there are), or no weights: grad_weights is None."""
+    g = _rows(grad_out, "grad_out")
+    dev, (t, k) = g.device, g.shape
+    m = _map(row_of_slot, dev)
+    if m.shape[0] != t:
+        raise ValueError(f"row_of_slot of shape {list(m.shape)}: [{t}, top-k] expected")
+    w = _weights(topk_weights, m, dev)
+    topk = m.shape[1]
+    x = None
+    if rows is not None:
+        x = _rows(rows, "rows", (rows.shape[0], k), g.dtype, dev)
+        num_rows = x.shape[0]
+    elif num_rows is None:
+        num_rows = t * topk
+    grad_rows = _output(out, (num_rows, k), g.dtype, dev)
+    grad_w = torch.empty((t, topk), dtype=torch.float32, device=dev) if w is not None and x is not None else None
+    _call(dev, "mxmoe_unpermute_tokens_backward", g.data_ptr(), g.stride(0), None if x is None else x.data_ptr(), 0 if x is None else x.stride(0), num_rows, m.data_ptr(),
+          None if w is None else w.data_ptr(), _TYPES[g.dtype], t, topk, k, grad_rows.data_ptr(), out is not None, None if grad_w is None else grad_w.data_ptr())
+    return grad_rows, grad_w
+
+
+def route_topk_backward(grad_weights: torch.Tensor, router_logits: torch.Tensor, topk_ids: torch.Tensor, renormalise: bool = False) -> torch.Tensor:
+    """Gradient of `route_topk`'s weights [T, k] with respect to its logits [T, E], in the logits' dtype, for the experts that it chose (`topk_ids` int32 or int64 [T, k])."""
+    if router_logits.dim() != 2 or router_logits.dtype not in _TYPES:
+        raise ValueError(f"router logits of dtype {router_logits.dtype}, shape {list(router_logits.shape)}: fp16, fp32 or bf16 [tokens, experts] expected")
+    _on(router_logits, "router_logits", None)
+    dev, (t, e) = router_logits.device, router_logits.shape
+    if topk_ids.dim() != 2 or topk_ids.shape[0] != t or grad_weights.shape != topk_ids.shape:
+        raise ValueError(f"topk_ids of shape {list(topk_ids.shape)}, grad_weights of shape {list(grad_weights.shape)}: [{t}, top-k] expected of both")
+    if topk_ids.dtype != torch.int32 and topk_ids.dtype != torch.int64:
+        raise ValueError(f"topk_ids of dtype {topk_ids.dtype}: int32 or int64 expected")
+    _on(topk_ids, "topk_ids", dev)
+    _on(grad_weights, "grad_weights", dev)
+    ids = topk_ids if topk_ids.dtype == torch.int32 else topk_ids.clamp(-1, e).to(torch.int32)
+    ids = ids.contiguous()
+    logits, g = router_logits.contiguous(), grad_weights.to(torch.float32).contiguous()
+    out = torch.empty_like(logits)
+    _call(dev, "mxmoe_route_topk_backward", g.data_ptr(), logits.data_ptr(), _TYPES[logits.dtype], ids.data_ptr(), t, e, ids.shape[1], int(bool(renormalise)), out.data_ptr())
+    return out
+
+
+# ---- norms, gate and residual scale ----
+
+def _vector(w, name, k, dtype, dev):
+    """(tensor or None, dtype of the vectors so far)."""
+    if w is None:
+        return None, dtype
+    if w.shape != (k,) or w.dtype not in _TYPES or (dtype is not None and w.dtype != dtype):
+        raise ValueError(f"{name} of dtype {w.dtype}, shape {list(w.shape)}: [{k}] in fp16, fp32 or bf16 expected, all vectors of one dtype")
+    _on(w, name, dev)
+    return w.contiguous(), w.dtype
+
+
+def block_norm(x: torch.Tensor, weight: torch.Tensor | None = None, eps: float = 1e-6, out_dtype: torch.dtype | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """y = x / sqrt(mean(x^2) + eps) * weight over rows [T, K], in `out_dtype` (default x's): from a bfloat16 or fp32 residual stream into the fp16 layer in one pass."""
+    if _recorded(x, weight, out=out):
+        return _Norm.apply(x, weight, eps, out_dtype)
+    xr = _rows(x, "x")
+    dev, (t, k) = xr.device, xr.shape
+    w, wt = _vector(weight, "weight", k, None, dev)
+    od = xr.dtype if out_dtype is None else out_dtype
+    if od not in _TYPES:
+        raise ValueError(_NO_TYPE.format("output", od))
+    y = _output(out, (t, k), od, dev)
+    _call(dev, "mxmoe_block_norm", xr.data_ptr(), xr.stride(0), _TYPES[xr.dtype], None if w is None else w.data_ptr(), 1 if wt is None else _TYPES[wt], eps, t, k, y.data_ptr(), _TYPES[od])
+    return y
+
+
+def block_norm_backward(grad_y: torch.Tensor, x: torch.Tensor, weight: torch.Tensor | None = None, eps: float = 1e-6, grad_residual: torch.Tensor | None = None):
+    """Gradients of `block_norm` -> (grad_x, grad_weight or None).  `grad_residual` [T, K] (x's dtype), the gradient that reaches x past the norm, is added to grad_x."""
+    xr = _rows(x, "x")
+    dev, (t, k) = xr.device, xr.shape
+    gy = _rows(grad_y, "grad_y", (t, k), None, dev)
+    gr = None if grad_residual is None else _rows(grad_residual, "grad_residual", (t, k), xr.dtype, dev)
+    w, wt = _vector(weight, "weight", k, None, dev)
+    grad_x = torch.empty((t, k), dtype=xr.dtype, device=dev)
+    grad_w, ws = (None, None) if w is None else (torch.empty_like(w), _workspace(t, k, dev))
+    _call(dev, "mxmoe_block_norm_backward", gy.data_ptr(), gy.stride(0), _TYPES[gy.dtype], xr.data_ptr(), xr.stride(0), _TYPES[xr.dtype], None if w is None else w.data_ptr(),
+          1 if wt is None else _TYPES[wt], None if gr is None else gr.data_ptr(), 0 if gr is None else gr.stride(0), eps, t, k, grad_x.data_ptr(), None if w is None else grad_w.data_ptr(),
+          None if ws is None else ws.data_ptr())
+    return grad_x, grad_w
+
+
+def _workspace(t, k, dev):
+    return torch.empty(_lib.load().mxmoe_block_backward_workspace_bytes(t, k), dtype=torch.uint8, device=dev)
+
+
+def _gate(gate, gate_act, z, dev):
+    """(kind, tensor or None, stride, dtype, sigmoid)."""
+    if gate_act not in (None, "sigmoid"):
+        raise ValueError(f"gate_act {gate_act!r}: None or 'sigmoid' expected")
+    if gate is None:
+        return 0, None, 0, 1, 0
+    t, k = z.shape
+    if gate.shape == (t,) or gate.shape == (t, 1):
+        if gate.dtype not in _TYPES:
+            raise ValueError(_NO_TYPE.format("gate", gate.dtype))
+        _on(gate, "gate", dev)
+        return 1, gate, gate.stride(0), _TYPES[gate.dtype], int(gate_act is not None)
+    if gate.shape != (t, k):
+        raise ValueError(f"gate of shape {list(gate.shape)}: [{t}], [{t}, 1] or [{t}, {k}] expected")
+    gate = _rows(gate, "gate", (t, k), z.dtype, dev)
+    return 2, gate, gate.stride(0), _TYPES[gate.dtype], int(gate_act is not None)
+
+
+def _residual_inputs(x, z, gate, gate_act, scale, norm_weight, next_weight):
+    xr = _rows(x, "x")
+    dev, (t, k) = xr.device, xr.shape
+    zr = _rows(z, "z", (t, k), None, dev)
+    kind, g, ldg, gt, sigmoid = _gate(gate, gate_act, zr, dev)
+    factor, vec = 1.0, None
+    if isinstance(scale, torch.Tensor):
+        vec = scale
+    elif scale is not None:
+        factor = float(scale)
+    vec, wt = _vector(vec, "scale", k, None, dev)
+    w1, wt = _vector(norm_weight, "norm_weight", k, wt, dev)
+    w2, wt = _vector(next_weight, "next_weight", k, wt, dev)
+    args = (xr.data_ptr(), xr.stride(0), _TYPES[xr.dtype], zr.data_ptr(), zr.stride(0), _TYPES[zr.dtype], kind, None if g is None else g.data_ptr(), ldg, gt, sigmoid, factor,
+            None if vec is None else vec.data_ptr(), None if w1 is None else w1.data_ptr(), None if w2 is None else w2.data_ptr(), 1 if wt is None else _TYPES[wt])
+    return args, (xr, zr, g, vec, w1, w2)
+
+
+def block_residual(x: torch.Tensor, z: torch.Tensor, *, gate: torch.Tensor | None = None, gate_act: str | None = None, scale: float | torch.Tensor | None = None,
+                   norm_weight: torch.Tensor | None = None, next_weight: torch.Tensor | None = None, eps: float = 1e-6, out: torch.Tensor | None = None):
+    """A block's output z [T, K] onto the residual stream x [T, K]: h = x + scale * gate * norm(z), in x's dtype; with `next_weight` -> (h, y), y = the next block's norm
+    of h in z's dtype, from the same pass.
+
+    norm(z) = z / sqrt(mean(z^2) + eps) * norm_weight, or z itself without `norm_weight`.  `gate` per token ([T] or [T, 1]) or per element ([T, K], z's dtype), through a
+    sigmoid with gate_act="sigmoid" (a shared expert's gate, say).  `scale`: a number, or one per channel [K].  The vectors have one dtype.  Everything is fp32 inside; y
+    is computed from h before its rounding.  `out` (x itself is allowed) receives h."""
+    if _recorded(x, z, gate, scale, norm_weight, next_weight, out=out):
+        vec, factor = (scale, None) if isinstance(scale, torch.Tensor) else (None, scale)
+        h, y = _Residual.apply(x, z, gate, vec, norm_weight, next_weight, gate_act, factor, eps)
+        return h if next_weight is None else (h, y)
+    args, (xr, zr, *keep) = _residual_inputs(x, z, gate, gate_act, scale, norm_weight, next_weight)
+    t, k = xr.shape
+    if out is not None and xr is not x and out.data_ptr() == x.data_ptr():
+        raise ValueError("out may be x only where x's elements lie side by side")
+    h = _output(out, (t, k), xr.dtype, xr.device)
+    y = None if next_weight is None else torch.empty((t, k), dtype=zr.dtype, device=xr.device)
+    _call(xr.device, "mxmoe_block_residual", *args, eps, t, k, h.data_ptr(), None if y is None else y.data_ptr())
+    return h if y is None else (h, y)
+
+
+def block_residual_backward(grad_h: torch.Tensor | None, grad_y: torch.Tensor | None, x: torch.Tensor, z: torch.Tensor, *, gate: torch.Tensor | None = None, gate_act: str | None = None,
+                            scale: float | torch.Tensor | None = None, norm_weight: torch.Tensor | None = None, next_weight: torch.Tensor | None = None, eps: float = 1e-6):
+    """Gradients of `block_residual` -> (grad_x, grad_z, grad_gate, grad_scale, grad_norm_weight, grad_next_weight), None for inputs that were not given or are numbers.
+    grad_h (x's dtype) or grad_y (z's dtype) may be None.  Nothing is kept from the forward call."""
+    args, (xr, zr, g, vec, w1, w2) = _residual_inputs(x, z, gate, gate_act, scale, norm_weight, next_weight)
+    dev, (t, k) = xr.device, xr.shape
+    if grad_y is not None and next_weight is None:
+        raise ValueError("grad_y without next_weight: the call had no y")
+    if grad_h is None and grad_y is None:
+        raise ValueError("neither grad_h nor grad_y is given")
+    gh = None if grad_h is None else _rows(grad_h, "grad_h", (t, k), xr.dtype, dev)
+    gy = None if grad_y is None else _rows(grad_y, "grad_y", (t, k), zr.dtype, dev)
+    grad_x, grad_z = torch.empty((t, k), dtype=xr.dtype, device=dev), torch.empty((t, k), dtype=zr.dtype, device=dev)
+    grad_gate = None if g is None else torch.empty(gate.shape, dtype=gate.dtype, device=dev)
+    grads = [None if w is None else torch.empty_like(w) for w in (vec, w1, w2)]
+    ws = None if all(w is None for w in grads) else _workspace(t, k, dev)
+    ptr = [None if w is None else w.data_ptr() for w in (gh, gy, grad_gate, *grads, ws)]
+    _call(dev, "mxmoe_block_residual_backward", ptr[0], 0 if gh is None else gh.stride(0), ptr[1], 0 if gy is None else gy.stride(0), *args, eps, t, k, grad_x.data_ptr(),
+          grad_z.data_ptr(), *ptr[2:])
+    return grad_x, grad_z, grad_gate, *grads
+
+
+# ---- the same for autograd ----
+
+class _Permute(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, hidden, topk_ids, num_experts, perm):
+        rows, row_of_slot, recv = _permute(hidden, topk_ids, num_experts, None, perm)
+        ctx.save_for_backward(row_of_slot)
+        ctx.mark_non_differentiable(row_of_slot, recv)
+        return rows, row_of_slot, recv
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_rows, _map, _recv):
+        return permute_tokens_backward(grad_rows, *ctx.saved_tensors), None, None, None
+
+
+class _Unpermute(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, rows, row_of_slot, topk_weights, shared):
+        ctx.save_for_backward(rows, row_of_slot, topk_weights)
+        return unpermute_tokens(rows, row_of_slot, topk_weights, shared)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_out):
+        rows, m, w = ctx.saved_tensors
+        need_rows, _, need_w, need_shared = ctx.needs_input_grad
+        grad_rows = grad_w = None
+        if need_rows or need_w:
+            grad_rows, grad_w = unpermute_tokens_backward(grad_out, rows if need_w else None, m, w, num_rows=rows.shape[0])
+        return grad_rows if need_rows else None, None, grad_w.to(w.dtype) if need_w else None, grad_out if need_shared else None
+
+
+class _Norm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, eps, out_dtype):
+        ctx.save_for_backward(x, weight)
+        ctx.eps = eps
+        return block_norm(x, weight, eps, out_dtype)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_y):
+        x, weight = ctx.saved_tensors
+        return *block_norm_backward(grad_y, x, weight, ctx.eps), None, None
+
+
+class _Residual(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, z, gate, scale, norm_weight, next_weight, gate_act, factor, eps):
+        ctx.save_for_backward(x, z, gate, scale, norm_weight, next_weight)
+        ctx.set_materialize_grads(False)
+        ctx.rest = gate_act, factor, eps
+        got = block_residual(x, z, gate=gate, gate_act=gate_act, scale=factor if scale is None else scale, norm_weight=norm_weight, next_weight=next_weight, eps=eps)
+        return got if next_weight is not None else (got, None)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_h, grad_y):
+        x, z, gate, scale, w1, w2 = ctx.saved_tensors
+        if grad_h is None and grad_y is None:
+            return (None,) * 9
+        gate_act, factor, eps = ctx.rest
+        grads = block_residual_backward(grad_h, grad_y, x, z, gate=gate, gate_act=gate_act, scale=factor if scale is None else scale, norm_weight=w1, next_weight=w2, eps=eps)
+        return *grads, None, None, None
+
+
+class RouteTopk(torch.autograd.Function):
+    """(ids, weights) of `route_topk`, the weights differentiable with respect to the logits."""
+
+    @staticmethod
+    def forward(ctx, logits, topk, renormalise):
+        from .ops import route_topk
+
+        ids, weights = route_topk(logits, topk, renormalise)
+        ctx.save_for_backward(logits, ids)
+        ctx.renormalise = renormalise
+        ctx.mark_non_differentiable(ids)
+        return ids, weights
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, _ids, grad_weights):
+        return route_topk_backward(grad_weights, *ctx.saved_tensors, renormalise=ctx.renormalise), None, None

@@ -1,0 +1,201 @@
+// Norms before and after a block fused with its gate and residual scale, forward (formulas: mxmoe_block_norm.hpp).
+//
+// One workgroup a row, the row in registers between its sums: one pass over x, z and the gate, one over h and y.  Bound by memory.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include <string>
+
+#include "../../include/mxmoe_amd.h"
+#include "include/mxmoe_block_norm.hpp"
+#include "include/mxmoe_launch.hpp"
+
+namespace mxmoe {
+
+template <typename TX, typename TZ, bool HAS_Z, int NT, int VPT>
+__global__ void __launch_bounds__(NT) block_norm_kernel(const BlockNormArgs a) {
+  __shared__ float sums[2][NT / 64];
+  const int K = a.K, C = (K + 7) >> 3;
+  const long t = blockIdx.x;
+  typename Piece<TX>::raw x_raw[VPT];
+  typename Piece<TZ>::raw z_raw[HAS_Z ? VPT : 1], g_raw[HAS_Z ? VPT : 1];
+#pragma unroll
+  for (int v = 0; v < VPT; ++v) {
+    const int c = threadIdx.x + v * NT;
+    if (c < C) {
+      x_raw[v] = load_piece(reinterpret_cast<const TX*>(a.x) + t * a.ldx, c, K);
+      if constexpr (HAS_Z) {
+        z_raw[v] = load_piece(reinterpret_cast<const TZ*>(a.z) + t * a.ldz, c, K);
+        if (a.gate_kind == kElementGate) g_raw[v] = load_piece(reinterpret_cast<const TZ*>(a.gate) + t * a.ldg, c, K);
+      }
+    } else {
+      x_raw[v] = 0;
+      if constexpr (HAS_Z) z_raw[v] = 0;
+    }
+  }
+  f8 h[VPT];
+#pragma unroll
+  for (int v = 0; v < VPT; ++v) h[v] = Piece<TX>::widen(x_raw[v]);
+  if constexpr (HAS_Z) {
+    float row = a.factor;  // what the whole row is multiplied by: the residual scale, a token's gate, r_z
+    if (a.gate_kind == kTokenGate) {
+      const float g = load_of(a.gate_type, a.gate, t * a.ldg);
+      row *= a.sigmoid ? sigmoid_of(g) : g;
+    }
+    if (a.w1) {
+      float sq[1] = {0.0f};
+#pragma unroll
+      for (int v = 0; v < VPT; ++v) {
+        const f8 z = Piece<TZ>::widen(z_raw[v]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sq[0] = __builtin_fmaf(z[e], z[e], sq[0]);
+      }
+      group_sum<NT, 1>(sq, sums[0]);
+      row *= rms_factor(sq[0], K, a.eps);
+    }
+#pragma unroll
+    for (int v = 0; v < VPT; ++v) {
+      const int c = threadIdx.x + v * NT;
+      if (c < C) {
+        f8 n = row * Piece<TZ>::widen(z_raw[v]);
+        if (a.w1) n *= load_piece_of(a.wtype, a.w1, c, K);
+        if (a.scale) n *= load_piece_of(a.wtype, a.scale, c, K);
+        if (a.gate_kind == kElementGate) {
+          const f8 g = Piece<TZ>::widen(g_raw[v]);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) n[e] *= a.sigmoid ? sigmoid_of(g[e]) : g[e];
+        }
+        h[v] += n;
+        store_piece(reinterpret_cast<TX*>(a.h) + t * K, c, K, Piece<TX>::narrow(h[v]));
+      }
+    }
+  }
+  if (HAS_Z && !a.y) return;
+  float sq[1] = {0.0f};
+#pragma unroll
+  for (int v = 0; v < VPT; ++v) {
+    const int c = threadIdx.x + v * NT;
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (8 * c + e < K) sq[0] = __builtin_fmaf(h[v][e], h[v][e], sq[0]);  // (past the row's end a gate may have left anything)
+  }
+  group_sum<NT, 1>(sq, sums[1]);
+  const float r = rms_factor(sq[0], K, a.eps);
+#pragma unroll
+  for (int v = 0; v < VPT; ++v) {
+    const int c = threadIdx.x + v * NT;
+    if (c < C) {
+      f8 y = r * h[v];
+      if (a.w2) y *= load_piece_of(a.wtype, a.w2, c, K);
+      store_piece(reinterpret_cast<TZ*>(a.y) + t * K, c, K, Piece<TZ>::narrow(y));
+    }
+  }
+}
+
+template <typename TX, typename TZ, bool HAS_Z>
+static void run_block_norm(const BlockNormArgs& a, hipStream_t s) {
+  const int C = (a.K + 7) / 8;
+  // threads a row: one wave up to 128 pieces (no barrier), then four waves, for very long rows sixteen
+#define RUN(NT, VPT) hipLaunchKernelGGL((block_norm_kernel<TX, TZ, HAS_Z, NT, VPT>), dim3(a.T), dim3(NT), 0, s, a)
+  if (C <= 128) RUN(64, 2);
+  else if (C <= 256) RUN(256, 1);
+  else if (C <= 512) RUN(256, 2);
+  else if (C <= 1024) RUN(256, 4);
+  else RUN(1024, 4);
+#undef RUN
+}
+template <typename TX, bool HAS_Z>
+static void run_block_norm_z(int ztype, const BlockNormArgs& a, hipStream_t s) {
+  if (ztype == kF16) run_block_norm<TX, _Float16, HAS_Z>(a, s);
+  else if (ztype == kF32) run_block_norm<TX, float, HAS_Z>(a, s);
+  else run_block_norm<TX, __bf16, HAS_Z>(a, s);
+}
+template <bool HAS_Z>
+static int run_block_norm_as(int xtype, int ztype, const BlockNormArgs& a, hipStream_t s) {
+  if (xtype == kF16) run_block_norm_z<_Float16, HAS_Z>(ztype, a, s);
+  else if (xtype == kF32) run_block_norm_z<float, HAS_Z>(ztype, a, s);
+  else run_block_norm_z<__bf16, HAS_Z>(ztype, a, s);
+  const hipError_t e = hipGetLastError();
+  if (e == hipSuccess) return 0;
+  last_error() = std::string("kernel launch failed: ") + hipGetErrorString(e);
+  return 4;
+}
+
+int check_block_norm(const BlockNormArgs& a, int xtype, int ztype) {
+  if (a.T < 0 || a.K < 1 || a.K > kMaxNormRow || a.ldx < 0 || a.ldz < 0 || a.ldg < 0 || a.ldgh < 0 || a.ldgy < 0) {
+    last_error() = "block norms take rows of 1 .. 32768 elements, tokens and row strides >= 0";
+    return 3;
+  }
+  if (xtype < 0 || xtype > 2 || ztype < 0 || ztype > 2 || a.wtype < 0 || a.wtype > 2 || a.gate_type < 0 || a.gate_type > 2 || a.gate_kind < 0 || a.gate_kind > 2) {
+    last_error() = "float types are fp16 (0), fp32 (1) or bf16 (2), gates none (0), per token (1) or per element (2)";
+    return 3;
+  }
+  if (a.T && a.gate_kind && !a.gate) {
+    last_error() = "null pointer";
+    return 5;
+  }
+  return 0;
+}
+
+}  // namespace mxmoe
+
+using namespace mxmoe;
+
+extern "C" {
+
+int mxmoe_block_norm(const void* x, int64_t ldx, int x_dtype, const void* weight, int weight_dtype, float eps, int num_tokens, int K, void* y, int y_dtype, void* stream) {
+  BlockNormArgs a{};
+  a.x = x;
+  a.ldx = (long)ldx;
+  a.w2 = weight;
+  a.wtype = weight_dtype;
+  a.eps = eps;
+  a.T = num_tokens;
+  a.K = K;
+  a.y = y;
+  if (const int rc = check_block_norm(a, x_dtype, y_dtype)) return rc;
+  if (num_tokens == 0) return 0;
+  if (!x || !y) {
+    last_error() = "null pointer";
+    return 5;
+  }
+  return run_block_norm_as<false>(x_dtype, y_dtype, a, (hipStream_t)stream);
+}
+
+int mxmoe_block_residual(const void* x, int64_t ldx, int x_dtype, const void* z, int64_t ldz, int z_dtype, int gate_kind, const void* gate, int64_t ld_gate, int gate_dtype, int sigmoid,
+                         float factor, const void* scale, const void* norm_weight, const void* next_weight, int weight_dtype, float eps, int num_tokens, int K, void* h, void* y,
+                         void* stream) {
+  BlockNormArgs a{};
+  a.x = x;
+  a.z = z;
+  a.gate = gate;
+  a.scale = scale;
+  a.w1 = norm_weight;
+  a.w2 = next_weight;
+  a.ldx = (long)ldx;
+  a.ldz = (long)ldz;
+  a.ldg = (long)ld_gate;
+  a.T = num_tokens;
+  a.K = K;
+  a.wtype = weight_dtype;
+  a.gate_kind = gate_kind;
+  a.gate_type = gate_dtype;
+  a.sigmoid = sigmoid != 0;
+  a.eps = eps;
+  a.factor = factor;
+  a.h = h;
+  a.y = y;
+  if (const int rc = check_block_norm(a, x_dtype, z_dtype)) return rc;
+  if (gate_kind == kElementGate && gate_dtype != z_dtype) {
+    last_error() = "a gate per element has the block output's type";
+    return 3;
+  }
+  if (num_tokens == 0) return 0;
+  if (!x || !z || !h) {
+    last_error() = "null pointer";
+    return 5;
+  }
+  return run_block_norm_as<true>(x_dtype, z_dtype, a, (hipStream_t)stream);
+}
+
+}  // extern "C"

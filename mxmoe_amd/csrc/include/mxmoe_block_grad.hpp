@@ -1,0 +1,219 @@
+// Backward kernel of the norms around a block (forward and notation: mxmoe_block_norm.hpp), instantiated per type of the residual stream.
+//
+//   c1  = r_h^3 / K  sum grad_y w2 h                     D  = grad_h + r_h grad_y w2 - c1 h            (grad_x = D)
+//   c2  = sum D s n (gate per element inside, per token outside the sum)
+//   grad_z    = r_z (D s a w1 - z r_z  c2 a_token / K)   or D s a without a norm behind the block
+//   grad_gate = c2 act' per token,  D s n act' per element
+//   P   = sum over tokens of grad_y h r_h                (grad_w2 = P)
+//   Q   = sum over tokens of D a z r_z                   (grad_w1 = s Q, grad_scale = factor w1 Q: one sum serves both)
+//
+// Nothing is kept from the forward pass: r_z and h are computed again from x and z, which the gradients read anyway.  That takes a sum over the row for r_z
+// and, behind it, five sums at once (h^2, grad_y w2 h and the three that c2 is made of), so a row costs two barriers.
+//
+// A workgroup works off every gridDim-th token and holds P and Q of its columns in registers; each workgroup writes them once and a second launch adds them up in a fixed
+// order.  The next token's pieces are on their way while the present one's sums wait at the barriers.
+#pragma once
+#include "mxmoe_block_norm.hpp"
+
+namespace mxmoe {
+
+template <typename TX, typename TZ, bool HAS_Z, int VPT>
+struct BackwardRow {
+  typename Piece<TX>::raw x[VPT], gh[VPT];
+  typename Piece<TZ>::raw gy[VPT], z[HAS_Z ? VPT : 1], g[HAS_Z ? VPT : 1];
+
+  template <int NT>
+  __device__ __forceinline__ void load(const BlockNormArgs& a, long t) {
+#pragma unroll
+    for (int v = 0; v < VPT; ++v) {
+      const int c = threadIdx.x + v * NT;
+      x[v] = 0;
+      gh[v] = 0;
+      gy[v] = 0;
+      if constexpr (HAS_Z) z[v] = g[v] = 0;
+      if (8 * c < a.K) {
+        x[v] = load_piece(reinterpret_cast<const TX*>(a.x) + t * a.ldx, c, a.K);
+        if constexpr (HAS_Z) {
+          z[v] = load_piece(reinterpret_cast<const TZ*>(a.z) + t * a.ldz, c, a.K);
+          if (a.gate_kind == kElementGate) g[v] = load_piece(reinterpret_cast<const TZ*>(a.gate) + t * a.ldg, c, a.K);
+        }
+        if (a.grad_h) gh[v] = load_piece(reinterpret_cast<const TX*>(a.grad_h) + t * a.ldgh, c, a.K);
+        if (a.grad_y) gy[v] = load_piece(reinterpret_cast<const TZ*>(a.grad_y) + t * a.ldgy, c, a.K);
+      }
+    }
+  }
+};
+
+__device__ __forceinline__ float dot8(f8 a, f8 b, float s) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) s = __builtin_fmaf(a[e], b[e], s);
+  return s;
+}
+
+template <typename TX, typename TZ, bool HAS_Z, int NT, int VPT>
+__global__ void __launch_bounds__(NT) block_norm_backward_kernel(const BlockNormArgs a) {
+  constexpr int W = NT / 64;
+  __shared__ float sums_z[2][W], sums_h[2][5 * W];
+  constexpr bool KEEP = VPT == 1;  // weights, and the next row's pieces, in registers
+  const int K = a.K;
+  const float inv_k = 1.0f / (float)K;
+  auto weight = [&](const void* w, int v) {
+    const int c = threadIdx.x + v * NT;
+    f8 r = 0.0f;
+    if (8 * c < K) r = w ? load_piece_of(a.wtype, w, c, K) : (f8)1.0f;
+    return r;
+  };
+  f8 w1_kept = 0.0f, w2_kept = 0.0f, s_kept = 0.0f;
+  if constexpr (KEEP) {
+    w2_kept = weight(a.w2, 0);
+    if constexpr (HAS_Z) {
+      w1_kept = weight(a.w1, 0);
+      s_kept = a.factor * weight(a.scale, 0);
+    }
+  }
+  f8 P[VPT], Q[HAS_Z ? VPT : 1];
+#pragma unroll
+  for (int v = 0; v < VPT; ++v) {
+    P[v] = 0.0f;
+    if constexpr (HAS_Z) Q[v] = 0.0f;
+  }
+  BackwardRow<TX, TZ, HAS_Z, VPT> next;
+  if constexpr (KEEP) next.template load<NT>(a, blockIdx.x);
+  int turn = 0;
+  for (long t = blockIdx.x; t < a.T; t += gridDim.x, turn ^= 1) {
+    BackwardRow<TX, TZ, HAS_Z, VPT> row;
+    if constexpr (KEEP) {
+      row = next;
+      if (t + gridDim.x < a.T) next.template load<NT>(a, t + gridDim.x);
+    } else {
+      row.template load<NT>(a, t);
+    }
+    float r_z = 1.0f, a_token = 1.0f, slope_token = 1.0f;
+    if constexpr (HAS_Z) {
+      if (a.gate_kind == kTokenGate) {
+        const float g = load_of(a.gate_type, a.gate, t * a.ldg);
+        a_token = a.sigmoid ? sigmoid_of(g) : g;
+        if (a.sigmoid) slope_token = sigmoid_slope(g);
+      }
+      if (a.w1) {
+        float sq[1] = {0.0f};
+#pragma unroll
+        for (int v = 0; v < VPT; ++v) {
+          const f8 z = Piece<TZ>::widen(row.z[v]);
+          sq[0] = dot8(z, z, sq[0]);
+        }
+        group_sum<NT, 1>(sq, sums_z[turn]);
+        r_z = rms_factor(sq[0], K, a.eps);
+      }
+    }
+    f8 h[VPT], sn[HAS_Z ? VPT : 1], act[HAS_Z ? VPT : 1];  // s n without a gate; the gate per element
+    float s[5] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int v = 0; v < VPT; ++v) {
+      h[v] = Piece<TX>::widen(row.x[v]);
+      f8 vn = 0.0f;
+      if constexpr (HAS_Z) {
+        sn[v] = r_z * Piece<TZ>::widen(row.z[v]) * (KEEP ? w1_kept : weight(a.w1, v)) * (KEEP ? s_kept : a.factor * weight(a.scale, v));
+        vn = sn[v];
+        if (a.gate_kind == kElementGate) {
+          act[v] = Piece<TZ>::widen(row.g[v]);
+          if (a.sigmoid) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) act[v][e] = sigmoid_of(act[v][e]);
+          }
+          vn *= act[v];
+        }
+        h[v] += a_token * vn;
+        s[2] = dot8(Piece<TX>::widen(row.gh[v]), vn, s[2]);
+      }
+      if (a.grad_y) {
+        const f8 dyw = Piece<TZ>::widen(row.gy[v]) * (KEEP ? w2_kept : weight(a.w2, v));
+        s[0] = dot8(h[v], h[v], s[0]);
+        s[1] = dot8(dyw, h[v], s[1]);
+        if constexpr (HAS_Z) {
+          s[3] = dot8(dyw, vn, s[3]);
+          s[4] = dot8(h[v], vn, s[4]);
+        }
+      }
+    }
+    float r_h = 0.0f, c1 = 0.0f, c2 = 0.0f;
+    if constexpr (HAS_Z) {
+      if (a.grad_y || a.w1 || a.gate_kind == kTokenGate) group_sum<NT, 5>(s, sums_h[turn]);
+    } else {
+      float two[2] = {s[0], s[1]};
+      group_sum<NT, 2>(two, sums_h[turn]);
+      s[0] = two[0];
+      s[1] = two[1];
+    }
+    if (a.grad_y) {
+      r_h = rms_factor(s[0], K, a.eps);
+      c1 = r_h * r_h * r_h * s[1] * inv_k;
+    }
+    if constexpr (HAS_Z) {
+      c2 = s[2] + r_h * s[3] - c1 * s[4];
+      if (a.gate_kind == kTokenGate && threadIdx.x == 0) store_of(a.gate_type, a.grad_gate, t, c2 * slope_token);
+    }
+#pragma unroll
+    for (int v = 0; v < VPT; ++v) {
+      const int c = threadIdx.x + v * NT;
+      const bool mine = 8 * c < K;
+      f8 D = Piece<TX>::widen(row.gh[v]);
+      if (a.grad_y) {
+        const f8 gy = Piece<TZ>::widen(row.gy[v]);
+        D += r_h * (gy * (KEEP ? w2_kept : weight(a.w2, v))) - c1 * h[v];
+        P[v] += gy * (r_h * h[v]);
+      }
+      if (mine) store_piece(reinterpret_cast<TX*>(a.grad_x) + t * K, c, K, Piece<TX>::narrow(D));
+      if constexpr (HAS_Z) {
+        const f8 zh = r_z * Piece<TZ>::widen(row.z[v]);
+        f8 Da = a_token * D;
+        if (a.gate_kind == kElementGate) {
+          f8 slope = 1.0f;
+          if (a.sigmoid) {
+            const f8 g = Piece<TZ>::widen(row.g[v]);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) slope[e] = sigmoid_slope(g[e]);
+          }
+          if (mine) store_piece(reinterpret_cast<TZ*>(a.grad_gate) + t * K, c, K, Piece<TZ>::narrow(D * sn[v] * slope));
+          Da *= act[v];
+        }
+        Q[v] += Da * zh;
+        f8 dz = Da * (KEEP ? s_kept : a.factor * weight(a.scale, v));
+        if (a.w1) dz = r_z * (dz * (KEEP ? w1_kept : weight(a.w1, v)) - zh * (a_token * c2 * inv_k));
+        if (mine) store_piece(reinterpret_cast<TZ*>(a.grad_z) + t * K, c, K, Piece<TZ>::narrow(dz));
+      }
+    }
+  }
+  float* mine = a.partial + (long)blockIdx.x * (HAS_Z ? 2 : 1) * K;
+#pragma unroll
+  for (int v = 0; v < VPT; ++v) {
+    const int c = threadIdx.x + v * NT;
+    if (8 * c < K) {
+      if (a.w2) store_piece(mine, c, K, P[v]);
+      if constexpr (HAS_Z) {
+        if (a.w1 || a.scale) store_piece(mine + K, c, K, Q[v]);
+      }
+    }
+  }
+}
+
+template <typename TX, typename TZ, bool HAS_Z>
+void run_block_backward_as(const BlockNormArgs& a, int grid, hipStream_t s) {
+#define RUN(NT, VPT) hipLaunchKernelGGL((block_norm_backward_kernel<TX, TZ, HAS_Z, NT, VPT>), dim3(grid), dim3(NT), 0, s, a)
+  if (a.K <= 512) RUN(64, 1);
+  else if (a.K <= 1024) RUN(128, 1);
+  else if (a.K <= 2048) RUN(256, 1);
+  else if (a.K <= 4096) RUN(512, 1);
+  else if (a.K <= 8192) RUN(1024, 1);
+  else if (a.K <= 16384) RUN(1024, 2);
+  else RUN(1024, 4);
+#undef RUN
+}
+template <typename TX>
+void run_block_backward(int ztype, bool has_z, const BlockNormArgs& a, int grid, hipStream_t s) {
+  if (ztype == kF16) has_z ? run_block_backward_as<TX, _Float16, true>(a, grid, s) : run_block_backward_as<TX, _Float16, false>(a, grid, s);
+  else if (ztype == kF32) has_z ? run_block_backward_as<TX, float, true>(a, grid, s) : run_block_backward_as<TX, float, false>(a, grid, s);
+  else has_z ? run_block_backward_as<TX, __bf16, true>(a, grid, s) : run_block_backward_as<TX, __bf16, false>(a, grid, s);
+}
+
+}  // namespace mxmoe

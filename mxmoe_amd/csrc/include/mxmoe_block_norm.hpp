@@ -1,0 +1,63 @@
+// The norms before and after a block, its gate and its residual scale: what the forward and the backward kernels share.
+//
+//   r_z = rsqrt(mean z^2 + eps), n = z r_z w1        (without a norm behind the block: n = z)
+//   a   = gate or sigmoid(gate), per token or per element      (1 without a gate)
+//   h   = x + s a n,  s = factor * scale[channel]
+//   r_h = rsqrt(mean h^2 + eps), y = h r_h w2        (the next block's norm; without z: h = x, a norm alone)
+//
+// h is rounded once on its way to memory; y comes from the unrounded h.
+#pragma once
+#include "mxmoe_vec8.hpp"
+
+namespace mxmoe {
+
+enum GateKind { kNoGate = 0, kTokenGate = 1, kElementGate = 2 };
+
+constexpr int kMaxNormRow = 32768;  // elements of a row: 1024 threads with four pieces each
+
+struct BlockNormArgs {
+  const void* x;
+  const void* z;
+  const void* gate;       // per token: [T], of gate_type; per element: rows of K, of z's type
+  const void* scale;      // [K], or null
+  const void* w1;         // [K], or null: no norm of z
+  const void* w2;         // [K], or null
+  long ldx, ldz, ldg;
+  int T, K;
+  int wtype, gate_kind, gate_type, sigmoid;
+  float eps, factor;
+  void* h;                // null with z null
+  void* y;                // null: no norm of h
+  // backward
+  const void* grad_h;     // null: no gradient of h (z null: none to be added)
+  const void* grad_y;     // null: no gradient of y
+  long ldgh, ldgy;
+  void* grad_x;
+  void* grad_z;
+  void* grad_gate;
+  float* partial;         // [grid][2][K]: sums over the workgroup's tokens of grad_y h r_h, and of grad_h' a z r_z
+};
+
+__device__ __forceinline__ float sigmoid_of(float g) { return 1.0f / (1.0f + expf(-g)); }
+// d sigmoid / dg = a (1 - a), from exp(-|g|): 1 - a would cancel where a is near 1
+__device__ __forceinline__ float sigmoid_slope(float g) {
+  const float e = expf(-fabsf(g));
+  return e / ((1.0f + e) * (1.0f + e));
+}
+// 1 / sqrt(sum / K + eps)
+__device__ __forceinline__ float rms_factor(float sum, int K, float eps) { return 1.0f / sqrtf(sum / (float)K + eps); }
+
+// Threads a row: one piece a thread up to rows of 8192, so that a workgroup's columns fit its registers.
+inline int backward_threads(int K) { return K <= 512 ? 64 : K <= 1024 ? 128 : K <= 2048 ? 256 : K <= 4096 ? 512 : 1024; }
+// Workgroups: as many as the card holds at once, each with the same number of tokens or one less
+inline int backward_groups(int T, int K) {
+  const int most = 131072 / backward_threads(K) < 256 ? 256 : 131072 / backward_threads(K);
+  return T < most ? T : (T + (T + most - 1) / most - 1) / ((T + most - 1) / most);
+}
+
+// one definition per type of x (block_norm_grad_*.hip)
+template <typename TX>
+void run_block_backward(int ztype, bool has_z, const BlockNormArgs& a, int grid, hipStream_t s);
+int check_block_norm(const BlockNormArgs& a, int xtype, int ztype);
+
+}  // namespace mxmoe

@@ -392,6 +392,20 @@ class MxMoELayer:
         ops.route_topk(router_logits.to(self.device), topk, renormalise, out_ids=ids, out_weights=w)
         return self(hidden, ids, w, out=out)
 
+    @torch.no_grad()
+    def forward_block(self, x: torch.Tensor, router_weight: torch.Tensor, norm_weight: torch.Tensor | None = None, *, normed: torch.Tensor | None = None, topk: int | None = None,
+                      renormalise: bool = False, gate: torch.Tensor | None = None, gate_act: str | None = None, scale: float | torch.Tensor | None = None,
+                      post_weight: torch.Tensor | None = None, next_weight: torch.Tensor | None = None, eps: float = 1e-6, out: torch.Tensor | None = None):
+        """The whole block on the residual stream x [T, K] (fp16, bf16 or fp32): `block_norm` into fp16, the router's logits (router_weight [E, K], a plain product in its
+        dtype), `forward_from_logits`, `block_residual` -> the new residual stream, with `next_weight` also the next block's normed input, which that block takes as
+        `normed` in place of its `norm_weight`.  gate, gate_act, scale, post_weight (the norm behind the block), out: as for `block_residual`.  Enqueues kernels only."""
+        if (normed is None) == (norm_weight is None):
+            raise ValueError("one of norm_weight and normed expected")
+        y = ops.block_norm(x, norm_weight, eps, out_dtype=torch.float16) if normed is None else normed
+        logits = torch.nn.functional.linear(y.to(router_weight.dtype), router_weight)
+        z = self.forward_from_logits(y, logits, topk, renormalise)
+        return ops.block_residual(x, z, gate=gate, gate_act=gate_act, scale=scale, norm_weight=post_weight, next_weight=next_weight, eps=eps, out=out)
+
     def capture(self, tokens: int, topk: int | None = None, logits_dtype: torch.dtype | None = None, renormalise: bool = False) -> "CapturedForward":
         """The planned forward for a fixed (tokens, top-k) shape, captured into a HIP graph: write the inputs into the returned
         object's `hidden`, `topk_ids`, `topk_weights` tensors, call `replay()`, read `out`.  Nothing in the forward depends on the

@@ -15,7 +15,9 @@ from functools import lru_cache
 import numpy as np
 import torch
 
-from . import _lib
+from . import _lib, block
+from .block import (block_norm, block_norm_backward, block_residual, block_residual_backward, permute_tokens, permute_tokens_backward,  # noqa: F401
+                    route_topk_backward, unpermute_tokens, unpermute_tokens_backward)
 from .group_gemm import GroupGemmLaunch, _upload
 from .hadamard import device_signs
 
@@ -93,6 +95,10 @@ def select_kernel(qparams, bf6: bool = False, fp8: bool = False, lib=None, bf16:
 
 def gg_permute_inp(hidden: torch.Tensor, topk_ids: torch.Tensor, E: int):
     """ref_bind.cu:47-64 -> (num_problems, inp_buffer [R, K], perm_indices [R], recv_tokens_per_exp [E] int64 CPU)."""
+    if hidden.dtype in _LOGIT_DTYPES and hidden.dim() == 2 and topk_ids.dtype in (torch.int32, torch.int64) and topk_ids.shape[1] <= 64:  # sort and copy in one pass
+        perm = torch.empty(topk_ids.numel(), dtype=torch.int64, device=topk_ids.device)
+        rows, recv_cpu = block.permute_with_indices(hidden, topk_ids, E, perm)
+        return int((recv_cpu != 0).sum()), rows[:int(recv_cpu.sum())], perm, recv_cpu
     dst, perm, _slot, recv = build_permutation(topk_ids, E)
     recv_cpu = recv.cpu()
     routed = int(recv_cpu.sum())                            # entries past this were never written (ids out of range are dropped)
@@ -110,7 +116,10 @@ _LOGIT_DTYPES = {torch.float16: 0, torch.float32: 1, torch.bfloat16: 2}
 def route_topk(router_logits: torch.Tensor, topk: int, renormalise: bool = False, out_ids: torch.Tensor | None = None, out_weights: torch.Tensor | None = None):
     """Router logits [T, E] (fp16, fp32 or bf16, on the device) -> (topk_ids int32 [T, k], topk_weights fp32 [T, k]): softmax over the
     experts in fp32, the k largest probabilities in decreasing order (equal ones: lower expert id first), divided by their sum when
-    `renormalise` (mxmoe/quant/moe_tracer.py:79-86).  `out_ids` / `out_weights` receive the result when given (no allocation)."""
+    `renormalise` (mxmoe/quant/moe_tracer.py:79-86).  `out_ids` / `out_weights` receive the result when given (no allocation).
+    Logits that require a gradient get it through the weights (`route_topk_backward`; not with `out_ids` / `out_weights`, nor under capture)."""
+    if out_ids is None and out_weights is None and block._recorded(router_logits):
+        return block.RouteTopk.apply(router_logits, topk, bool(renormalise))
     lib = _lib.load()
     if router_logits.dtype not in _LOGIT_DTYPES:
         raise ValueError(f"router logits of dtype {router_logits.dtype}: fp16, fp32 or bf16 expected")
