@@ -40,18 +40,17 @@ __global__ void __launch_bounds__(NT) block_norm_kernel(const BlockNormArgs a) {
     float row = a.factor;  // what the whole row is multiplied by: the residual scale, a token's gate, r_z
     if (a.gate_kind == kTokenGate) {
       const float g = load_of(a.gate_type, a.gate, t * a.ldg);
-      row *= a.sigmoid ? sigmoid_of(g) : g;
+      row *= a.sigmoid ? Sigmoid(g).a : g;
     }
     if (a.w1) {
       float sq[1] = {0.0f};
 #pragma unroll
       for (int v = 0; v < VPT; ++v) {
         const f8 z = Piece<TZ>::widen(z_raw[v]);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) sq[0] = __builtin_fmaf(z[e], z[e], sq[0]);
+        sq[0] = dot8(z, z, sq[0]);
       }
       group_sum<NT, 1>(sq, sums[0]);
-      row *= rms_factor(sq[0], K, a.eps);
+      row *= rms_factor(sq[0], 1.0f / (float)K, a.eps);
     }
 #pragma unroll
     for (int v = 0; v < VPT; ++v) {
@@ -63,7 +62,7 @@ __global__ void __launch_bounds__(NT) block_norm_kernel(const BlockNormArgs a) {
         if (a.gate_kind == kElementGate) {
           const f8 g = Piece<TZ>::widen(g_raw[v]);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) n[e] *= a.sigmoid ? sigmoid_of(g[e]) : g[e];
+          for (int e = 0; e < 8; ++e) n[e] *= a.sigmoid ? Sigmoid(g[e]).a : g[e];
         }
         h[v] += n;
         store_piece(reinterpret_cast<TX*>(a.h) + t * K, c, K, Piece<TX>::narrow(h[v]));
@@ -80,7 +79,7 @@ __global__ void __launch_bounds__(NT) block_norm_kernel(const BlockNormArgs a) {
       if (8 * c + e < K) sq[0] = __builtin_fmaf(h[v][e], h[v][e], sq[0]);  // (past the row's end a gate may have left anything)
   }
   group_sum<NT, 1>(sq, sums[1]);
-  const float r = rms_factor(sq[0], K, a.eps);
+  const float r = rms_factor(sq[0], 1.0f / (float)K, a.eps);
 #pragma unroll
   for (int v = 0; v < VPT; ++v) {
     const int c = threadIdx.x + v * NT;

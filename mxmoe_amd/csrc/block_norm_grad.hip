@@ -20,9 +20,9 @@ struct ColumnSumArgs {
   void* grad_w1;         // from plane 1
   void* grad_scale;
 };
-// 32 columns a workgroup (128 bytes of every partial row), eight threads a column.
-__global__ void __launch_bounds__(256) column_sum_kernel(const ColumnSumArgs a) {
-  __shared__ float part[8][33];
+// 32 columns a workgroup (128 bytes of every partial row), 32 threads a column: sixteen rows each of 512, in two rounds of loads.
+__global__ void __launch_bounds__(1024) column_sum_kernel(const ColumnSumArgs a) {
+  __shared__ float part[32][33];
   const int col = threadIdx.x & 31, sub = threadIdx.x >> 5, plane = blockIdx.y;
   if (plane == 0 ? !a.grad_w2 : !a.grad_w1 && !a.grad_scale) return;
   const int c = blockIdx.x * 32 + col;
@@ -31,13 +31,13 @@ __global__ void __launch_bounds__(256) column_sum_kernel(const ColumnSumArgs a) 
     const float* p = a.partial + (long)plane * a.K + c;
     const long ld = (long)a.planes * a.K;
 #pragma unroll 8
-    for (int g = sub; g < a.groups; g += 8) s += p[g * ld];
+    for (int g = sub; g < a.groups; g += 32) s += p[g * ld];
   }
   part[sub][col] = s;
   __syncthreads();
   if (sub || c >= a.K) return;
 #pragma unroll
-  for (int i = 1; i < 8; ++i) s += part[i][col];
+  for (int i = 1; i < 32; ++i) s += part[i][col];
   if (plane == 0) {
     store_of(a.wtype, a.grad_w2, c, s);
   } else {
@@ -56,7 +56,7 @@ static int run_backward(int xtype, int ztype, bool has_z, const BlockNormArgs& a
   if (grad_w2 || grad_w1 || grad_scale) {  // (no tokens: the sums are zero, and are written)
     const int planes = has_z ? 2 : 1;
     const ColumnSumArgs c{a.partial, grid, planes, a.K, a.wtype, a.factor, a.scale, a.w1, grad_w2, grad_w1, grad_scale};
-    hipLaunchKernelGGL(column_sum_kernel, dim3((a.K + 31) / 32, planes), dim3(256), 0, s, c);
+    hipLaunchKernelGGL(column_sum_kernel, dim3((a.K + 31) / 32, planes), dim3(1024), 0, s, c);
   }
   const hipError_t e = hipGetLastError();
   if (e == hipSuccess) return 0;

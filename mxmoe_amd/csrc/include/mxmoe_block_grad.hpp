@@ -17,7 +17,7 @@
 
 namespace mxmoe {
 
-template <typename TX, typename TZ, bool HAS_Z, int VPT>
+template <typename TX, typename TZ, bool HAS_Z, int VPT, bool WHOLE>
 struct BackwardRow {
   typename Piece<TX>::raw x[VPT], gh[VPT];
   typename Piece<TZ>::raw gy[VPT], z[HAS_Z ? VPT : 1], g[HAS_Z ? VPT : 1];
@@ -32,25 +32,19 @@ struct BackwardRow {
       gy[v] = 0;
       if constexpr (HAS_Z) z[v] = g[v] = 0;
       if (8 * c < a.K) {
-        x[v] = load_piece(reinterpret_cast<const TX*>(a.x) + t * a.ldx, c, a.K);
+        x[v] = load_piece<TX, WHOLE>(reinterpret_cast<const TX*>(a.x) + t * a.ldx, c, a.K);
         if constexpr (HAS_Z) {
-          z[v] = load_piece(reinterpret_cast<const TZ*>(a.z) + t * a.ldz, c, a.K);
-          if (a.gate_kind == kElementGate) g[v] = load_piece(reinterpret_cast<const TZ*>(a.gate) + t * a.ldg, c, a.K);
+          z[v] = load_piece<TZ, WHOLE>(reinterpret_cast<const TZ*>(a.z) + t * a.ldz, c, a.K);
+          if (a.gate_kind == kElementGate) g[v] = load_piece<TZ, WHOLE>(reinterpret_cast<const TZ*>(a.gate) + t * a.ldg, c, a.K);
         }
-        if (a.grad_h) gh[v] = load_piece(reinterpret_cast<const TX*>(a.grad_h) + t * a.ldgh, c, a.K);
-        if (a.grad_y) gy[v] = load_piece(reinterpret_cast<const TZ*>(a.grad_y) + t * a.ldgy, c, a.K);
+        if (a.grad_h) gh[v] = load_piece<TX, WHOLE>(reinterpret_cast<const TX*>(a.grad_h) + t * a.ldgh, c, a.K);
+        if (a.grad_y) gy[v] = load_piece<TZ, WHOLE>(reinterpret_cast<const TZ*>(a.grad_y) + t * a.ldgy, c, a.K);
       }
     }
   }
 };
 
-__device__ __forceinline__ float dot8(f8 a, f8 b, float s) {
-#pragma unroll
-  for (int e = 0; e < 8; ++e) s = __builtin_fmaf(a[e], b[e], s);
-  return s;
-}
-
-template <typename TX, typename TZ, bool HAS_Z, int NT, int VPT>
+template <typename TX, typename TZ, bool HAS_Z, int NT, int VPT, bool WHOLE>
 __global__ void __launch_bounds__(NT) block_norm_backward_kernel(const BlockNormArgs a) {
   constexpr int W = NT / 64;
   __shared__ float sums_z[2][W], sums_h[2][5 * W];
@@ -60,16 +54,15 @@ __global__ void __launch_bounds__(NT) block_norm_backward_kernel(const BlockNorm
   auto weight = [&](const void* w, int v) {
     const int c = threadIdx.x + v * NT;
     f8 r = 0.0f;
-    if (8 * c < K) r = w ? load_piece_of(a.wtype, w, c, K) : (f8)1.0f;
+    if (8 * c < K) r = w ? load_piece_of<WHOLE>(a.wtype, w, c, K) : f8(1.0f);
     return r;
   };
-  f8 w1_kept = 0.0f, w2_kept = 0.0f, s_kept = 0.0f;
+  auto next_weight = [&](int v) { return weight(a.w2, v); };
+  auto block_weight = [&](int v) { return a.factor * weight(a.scale, v) * weight(a.w1, v); };  // s w1: all that grad_z and c2 need of the two
+  f8 w2_kept = 0.0f, sw_kept = 0.0f;
   if constexpr (KEEP) {
-    w2_kept = weight(a.w2, 0);
-    if constexpr (HAS_Z) {
-      w1_kept = weight(a.w1, 0);
-      s_kept = a.factor * weight(a.scale, 0);
-    }
+    w2_kept = next_weight(0);
+    if constexpr (HAS_Z) sw_kept = block_weight(0);
   }
   f8 P[VPT], Q[HAS_Z ? VPT : 1];
 #pragma unroll
@@ -77,11 +70,11 @@ __global__ void __launch_bounds__(NT) block_norm_backward_kernel(const BlockNorm
     P[v] = 0.0f;
     if constexpr (HAS_Z) Q[v] = 0.0f;
   }
-  BackwardRow<TX, TZ, HAS_Z, VPT> next;
+  BackwardRow<TX, TZ, HAS_Z, VPT, WHOLE> next;
   if constexpr (KEEP) next.template load<NT>(a, blockIdx.x);
   int turn = 0;
   for (long t = blockIdx.x; t < a.T; t += gridDim.x, turn ^= 1) {
-    BackwardRow<TX, TZ, HAS_Z, VPT> row;
+    BackwardRow<TX, TZ, HAS_Z, VPT, WHOLE> row;
     if constexpr (KEEP) {
       row = next;
       if (t + gridDim.x < a.T) next.template load<NT>(a, t + gridDim.x);
@@ -89,54 +82,66 @@ __global__ void __launch_bounds__(NT) block_norm_backward_kernel(const BlockNorm
       row.template load<NT>(a, t);
     }
     float r_z = 1.0f, a_token = 1.0f, slope_token = 1.0f;
+    f8 zh[HAS_Z ? VPT : 1];  // z, then z r_z
     if constexpr (HAS_Z) {
       if (a.gate_kind == kTokenGate) {
         const float g = load_of(a.gate_type, a.gate, t * a.ldg);
-        a_token = a.sigmoid ? sigmoid_of(g) : g;
-        if (a.sigmoid) slope_token = sigmoid_slope(g);
+        a_token = g;
+        if (a.sigmoid) {
+          const Sigmoid s(g);
+          a_token = s.a;
+          slope_token = s.slope;
+        }
       }
+#pragma unroll
+      for (int v = 0; v < VPT; ++v) zh[v] = Piece<TZ>::widen(row.z[v]);
       if (a.w1) {
         float sq[1] = {0.0f};
 #pragma unroll
-        for (int v = 0; v < VPT; ++v) {
-          const f8 z = Piece<TZ>::widen(row.z[v]);
-          sq[0] = dot8(z, z, sq[0]);
-        }
+        for (int v = 0; v < VPT; ++v) sq[0] = dot8(zh[v], zh[v], sq[0]);
         group_sum<NT, 1>(sq, sums_z[turn]);
-        r_z = rms_factor(sq[0], K, a.eps);
+        r_z = rms_factor(sq[0], inv_k, a.eps);
+#pragma unroll
+        for (int v = 0; v < VPT; ++v) zh[v] *= r_z;
       }
     }
-    f8 h[VPT], sn[HAS_Z ? VPT : 1], act[HAS_Z ? VPT : 1];  // s n without a gate; the gate per element
+    f8 h[VPT], gh[VPT], gy[VPT], dyw[VPT], act[HAS_Z ? VPT : 1], steep[HAS_Z ? VPT : 1];  // dyw: grad_y w2; act: the gate per element; steep: s n times its slope
     float s[5] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int v = 0; v < VPT; ++v) {
       h[v] = Piece<TX>::widen(row.x[v]);
+      gh[v] = Piece<TX>::widen(row.gh[v]);
       f8 vn = 0.0f;
       if constexpr (HAS_Z) {
-        sn[v] = r_z * Piece<TZ>::widen(row.z[v]) * (KEEP ? w1_kept : weight(a.w1, v)) * (KEEP ? s_kept : a.factor * weight(a.scale, v));
-        vn = sn[v];
+        vn = zh[v] * (KEEP ? sw_kept : block_weight(v));
         if (a.gate_kind == kElementGate) {
           act[v] = Piece<TZ>::widen(row.g[v]);
+          steep[v] = vn;
           if (a.sigmoid) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) act[v][e] = sigmoid_of(act[v][e]);
+            for (int e = 0; e < 8; ++e) {
+              const Sigmoid s(act[v][e]);
+              act[v][e] = s.a;
+              steep[v][e] *= s.slope;
+            }
           }
           vn *= act[v];
         }
-        h[v] += a_token * vn;
-        s[2] = dot8(Piece<TX>::widen(row.gh[v]), vn, s[2]);
+        h[v] = fma8(a_token, vn, h[v]);
+        s[2] = dot8(gh[v], vn, s[2]);
       }
       if (a.grad_y) {
-        const f8 dyw = Piece<TZ>::widen(row.gy[v]) * (KEEP ? w2_kept : weight(a.w2, v));
+        gy[v] = Piece<TZ>::widen(row.gy[v]);
+        dyw[v] = gy[v] * (KEEP ? w2_kept : next_weight(v));
         s[0] = dot8(h[v], h[v], s[0]);
-        s[1] = dot8(dyw, h[v], s[1]);
+        s[1] = dot8(dyw[v], h[v], s[1]);
         if constexpr (HAS_Z) {
-          s[3] = dot8(dyw, vn, s[3]);
+          s[3] = dot8(dyw[v], vn, s[3]);
           s[4] = dot8(h[v], vn, s[4]);
         }
       }
     }
-    float r_h = 0.0f, c1 = 0.0f, c2 = 0.0f;
+    float r_h = 0.0f, c1 = 0.0f, c2 = 0.0f, c3 = 0.0f;
     if constexpr (HAS_Z) {
       if (a.grad_y || a.w1 || a.gate_kind == kTokenGate) group_sum<NT, 5>(s, sums_h[turn]);
     } else {
@@ -146,41 +151,36 @@ __global__ void __launch_bounds__(NT) block_norm_backward_kernel(const BlockNorm
       s[1] = two[1];
     }
     if (a.grad_y) {
-      r_h = rms_factor(s[0], K, a.eps);
+      r_h = rms_factor(s[0], inv_k, a.eps);
       c1 = r_h * r_h * r_h * s[1] * inv_k;
     }
     if constexpr (HAS_Z) {
       c2 = s[2] + r_h * s[3] - c1 * s[4];
+      if (a.w1) c3 = a_token * c2 * inv_k;
       if (a.gate_kind == kTokenGate && threadIdx.x == 0) store_of(a.gate_type, a.grad_gate, t, c2 * slope_token);
     }
 #pragma unroll
     for (int v = 0; v < VPT; ++v) {
       const int c = threadIdx.x + v * NT;
       const bool mine = 8 * c < K;
-      f8 D = Piece<TX>::widen(row.gh[v]);
+      f8 D = gh[v];
       if (a.grad_y) {
-        const f8 gy = Piece<TZ>::widen(row.gy[v]);
-        D += r_h * (gy * (KEEP ? w2_kept : weight(a.w2, v))) - c1 * h[v];
-        P[v] += gy * (r_h * h[v]);
+        D = fma8(r_h, dyw[v], fma8(-c1, h[v], D));
+        P[v] = fma8(gy[v], r_h * h[v], P[v]);
       }
-      if (mine) store_piece(reinterpret_cast<TX*>(a.grad_x) + t * K, c, K, Piece<TX>::narrow(D));
+      if (mine) store_piece<TX, WHOLE>(reinterpret_cast<TX*>(a.grad_x) + t * K, c, K, Piece<TX>::narrow(D));
       if constexpr (HAS_Z) {
-        const f8 zh = r_z * Piece<TZ>::widen(row.z[v]);
-        f8 Da = a_token * D;
+        f8 dz;
         if (a.gate_kind == kElementGate) {
-          f8 slope = 1.0f;
-          if (a.sigmoid) {
-            const f8 g = Piece<TZ>::widen(row.g[v]);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) slope[e] = sigmoid_slope(g[e]);
-          }
-          if (mine) store_piece(reinterpret_cast<TZ*>(a.grad_gate) + t * K, c, K, Piece<TZ>::narrow(D * sn[v] * slope));
-          Da *= act[v];
+          if (mine) store_piece<TZ, WHOLE>(reinterpret_cast<TZ*>(a.grad_gate) + t * K, c, K, Piece<TZ>::narrow(D * steep[v]));
+          D *= act[v];
+        } else if (a.gate_kind == kTokenGate) {
+          D *= a_token;
         }
-        Q[v] += Da * zh;
-        f8 dz = Da * (KEEP ? s_kept : a.factor * weight(a.scale, v));
-        if (a.w1) dz = r_z * (dz * (KEEP ? w1_kept : weight(a.w1, v)) - zh * (a_token * c2 * inv_k));
-        if (mine) store_piece(reinterpret_cast<TZ*>(a.grad_z) + t * K, c, K, Piece<TZ>::narrow(dz));
+        Q[v] = fma8(D, zh[v], Q[v]);
+        dz = D * (KEEP ? sw_kept : block_weight(v));
+        if (a.w1) dz = r_z * fma8(-c3, zh[v], dz);
+        if (mine) store_piece<TZ, WHOLE>(reinterpret_cast<TZ*>(a.grad_z) + t * K, c, K, Piece<TZ>::narrow(dz));
       }
     }
   }
@@ -189,9 +189,9 @@ __global__ void __launch_bounds__(NT) block_norm_backward_kernel(const BlockNorm
   for (int v = 0; v < VPT; ++v) {
     const int c = threadIdx.x + v * NT;
     if (8 * c < K) {
-      if (a.w2) store_piece(mine, c, K, P[v]);
+      if (a.w2) store_piece<float, WHOLE, kCached>(mine, c, K, Piece<float>::narrow(P[v]));
       if constexpr (HAS_Z) {
-        if (a.w1 || a.scale) store_piece(mine + K, c, K, Q[v]);
+        if (a.w1 || a.scale) store_piece<float, WHOLE, kCached>(mine + K, c, K, Piece<float>::narrow(Q[v]));
       }
     }
   }
@@ -199,14 +199,19 @@ __global__ void __launch_bounds__(NT) block_norm_backward_kernel(const BlockNorm
 
 template <typename TX, typename TZ, bool HAS_Z>
 void run_block_backward_as(const BlockNormArgs& a, int grid, hipStream_t s) {
-#define RUN(NT, VPT) hipLaunchKernelGGL((block_norm_backward_kernel<TX, TZ, HAS_Z, NT, VPT>), dim3(grid), dim3(NT), 0, s, a)
-  if (a.K <= 512) RUN(64, 1);
-  else if (a.K <= 1024) RUN(128, 1);
-  else if (a.K <= 2048) RUN(256, 1);
-  else if (a.K <= 4096) RUN(512, 1);
-  else if (a.K <= 8192) RUN(1024, 1);
-  else if (a.K <= 16384) RUN(1024, 2);
-  else RUN(1024, 4);
+#define RUN(NT, VPT, WHOLE) hipLaunchKernelGGL((block_norm_backward_kernel<TX, TZ, HAS_Z, NT, VPT, WHOLE>), dim3(grid), dim3(NT), 0, s, a)
+  if (a.K % 8) {  // (few sizes of workgroup: such rows are rare, their form only has to be there)
+    if (a.K <= 512) RUN(64, 1, false);
+    else if (a.K <= 2048) RUN(256, 1, false);
+    else if (a.K <= 8192) RUN(1024, 1, false);
+    else RUN(1024, 4, false);
+  } else if (a.K <= 512) RUN(64, 1, true);
+  else if (a.K <= 1024) RUN(128, 1, true);
+  else if (a.K <= 2048) RUN(256, 1, true);
+  else if (a.K <= 4096) RUN(512, 1, true);
+  else if (a.K <= 8192) RUN(1024, 1, true);
+  else if (a.K <= 16384) RUN(1024, 2, true);
+  else RUN(1024, 4, true);
 #undef RUN
 }
 template <typename TX>

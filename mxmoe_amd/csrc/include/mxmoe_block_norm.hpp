@@ -7,6 +7,8 @@
 //
 // h is rounded once on its way to memory; y comes from the unrounded h.
 #pragma once
+#include <algorithm>
+
 #include "mxmoe_vec8.hpp"
 
 namespace mxmoe {
@@ -38,20 +40,34 @@ struct BlockNormArgs {
   float* partial;         // [grid][2][K]: sums over the workgroup's tokens of grad_y h r_h, and of grad_h' a z r_z
 };
 
-__device__ __forceinline__ float sigmoid_of(float g) { return 1.0f / (1.0f + expf(-g)); }
-// d sigmoid / dg = a (1 - a), from exp(-|g|): 1 - a would cancel where a is near 1
-__device__ __forceinline__ float sigmoid_slope(float g) {
-  const float e = expf(-fabsf(g));
-  return e / ((1.0f + e) * (1.0f + e));
+// sigmoid(g) = 1 / (1 + exp(-g)) and its slope a (1 - a), both from e = exp(-|g|), which neither overflows nor lets 1 - a cancel: a = 1 / (1 + e) for g >= 0 and e / (1 + e)
+// below, slope = e / (1 + e)^2.  The exponential is 2^(x log2 e) with the product's rounding error put back to first order, the quotient the reciprocal
+// instruction's (one unit in the last place): 14 instructions for both, where expf and a division for each took some 45 and were half of the backward kernel's time.
+struct Sigmoid {
+  float a, slope;
+  __device__ __forceinline__ explicit Sigmoid(float g) {
+    constexpr float kLog2e = 1.44269504f, kLog2eLow = 1.92596303e-8f, kLn2 = 0.693147181f;
+    const float x = -fabsf(g), t = x * kLog2e;
+    const float low = __builtin_fmaf(x, kLog2eLow, __builtin_fmaf(x, kLog2e, -t));
+    float e = __builtin_amdgcn_exp2f(t);
+    e = x < -100.0f ? e : __builtin_fmaf(e * kLn2, low, e);  // (there e is below 4e-44, and -inf has no rounding error)
+    const float r = __builtin_amdgcn_rcpf(1.0f + e);
+    a = g < 0.0f ? e * r : r;
+    slope = e * r * r;
+  }
+};
+// 1 / sqrt(sum / K + eps), by the instruction (one unit in the last place) where its operand is far from the subnormal numbers, which it takes for zero
+__device__ __forceinline__ float rms_factor(float sum, float inv_k, float eps) {
+  const float v = sum * inv_k + eps;
+  if (v < 1e-30f) return 1.0f / sqrtf(v);
+  return __builtin_amdgcn_rsqf(v);
 }
-// 1 / sqrt(sum / K + eps)
-__device__ __forceinline__ float rms_factor(float sum, int K, float eps) { return 1.0f / sqrtf(sum / (float)K + eps); }
 
 // Threads a row: one piece a thread up to rows of 8192, so that a workgroup's columns fit its registers.
 inline int backward_threads(int K) { return K <= 512 ? 64 : K <= 1024 ? 128 : K <= 2048 ? 256 : K <= 4096 ? 512 : 1024; }
 // Workgroups: as many as the card holds at once, each with the same number of tokens or one less
 inline int backward_groups(int T, int K) {
-  const int most = 131072 / backward_threads(K) < 256 ? 256 : 131072 / backward_threads(K);
+  const int most = std::max(256, 131072 / backward_threads(K));
   return T < most ? T : (T + (T + most - 1) / most - 1) / ((T + most - 1) / most);
 }
 

@@ -10,7 +10,55 @@
 
 namespace mxmoe {
 
-typedef float f8 __attribute__((ext_vector_type(8)));
+// Eight values in registers of their own: a vector type of eight would hold eight neighbouring registers wherever it lives across a branch (175 registers instead of
+// REGS in the largest kernel).
+struct f8 {
+  float v[8];
+  f8() = default;
+  __device__ __forceinline__ f8(float x) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = x;
+  }
+  __device__ __forceinline__ float& operator[](int e) { return v[e]; }
+  __device__ __forceinline__ float operator[](int e) const { return v[e]; }
+};
+template <typename OP>
+__device__ __forceinline__ f8 each(const f8& a, const f8& b, OP op) {
+  f8 r;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) r.v[e] = op(a.v[e], b.v[e]);
+  return r;
+}
+__device__ __forceinline__ f8 operator+(const f8& a, const f8& b) { return each(a, b, [](float x, float y) { return x + y; }); }
+__device__ __forceinline__ f8 operator-(const f8& a, const f8& b) { return each(a, b, [](float x, float y) { return x - y; }); }
+__device__ __forceinline__ f8 operator*(const f8& a, const f8& b) { return each(a, b, [](float x, float y) { return x * y; }); }
+__device__ __forceinline__ f8& operator+=(f8& a, const f8& b) { return a = a + b; }
+__device__ __forceinline__ f8& operator*=(f8& a, const f8& b) { return a = a * b; }
+// a b + c, rounded once
+__device__ __forceinline__ f8 fma8(const f8& a, const f8& b, const f8& c) {
+  f8 r;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) r.v[e] = __builtin_fmaf(a.v[e], b.v[e], c.v[e]);
+  return r;
+}
+__device__ __forceinline__ float dot8(const f8& a, const f8& b, float s) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) s = __builtin_fmaf(a.v[e], b.v[e], s);
+  return s;
+}
+typedef float v8f __attribute__((ext_vector_type(8)));
+__device__ __forceinline__ f8 spread(v8f x) {
+  f8 r;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) r.v[e] = x[e];
+  return r;
+}
+__device__ __forceinline__ v8f gather(const f8& x) {
+  v8f r;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) r[e] = x.v[e];
+  return r;
+}
 
 // float types of the C entry points (as the routing's logits_dtype)
 enum FloatType { kF16 = 0, kF32 = 1, kBF16 = 2 };
@@ -23,30 +71,37 @@ template <>
 struct Piece<_Float16> {
   typedef _Float16 raw __attribute__((ext_vector_type(8)));
   typedef raw mem __attribute__((aligned(2)));
-  static __device__ __forceinline__ f8 widen(raw v) { return __builtin_convertvector(v, f8); }
-  static __device__ __forceinline__ raw narrow(f8 v) { return __builtin_convertvector(v, raw); }
+  static __device__ __forceinline__ f8 widen(raw v) { return spread(__builtin_convertvector(v, v8f)); }
+  static __device__ __forceinline__ raw narrow(const f8& v) { return __builtin_convertvector(gather(v), raw); }
 };
 template <>
 struct Piece<__bf16> {
   typedef __bf16 raw __attribute__((ext_vector_type(8)));
   typedef raw mem __attribute__((aligned(2)));
-  static __device__ __forceinline__ f8 widen(raw v) { return __builtin_convertvector(v, f8); }
-  static __device__ __forceinline__ raw narrow(f8 v) { return __builtin_convertvector(v, raw); }
+  static __device__ __forceinline__ f8 widen(raw v) { return spread(__builtin_convertvector(v, v8f)); }
+  static __device__ __forceinline__ raw narrow(const f8& v) { return __builtin_convertvector(gather(v), raw); }
 };
 template <>
 struct Piece<float> {
-  typedef f8 raw;
+  typedef v8f raw;
   typedef raw mem __attribute__((aligned(4)));
-  static __device__ __forceinline__ f8 widen(raw v) { return v; }
-  static __device__ __forceinline__ raw narrow(f8 v) { return v; }
+  static __device__ __forceinline__ f8 widen(raw v) { return spread(v); }
+  static __device__ __forceinline__ raw narrow(const f8& v) { return gather(v); }
 };
 
-// elements 8 c .. 8 c + 7 of a row of K elements, zeros past its end
-template <typename T>
+// How a piece goes through the caches.  Rows are read once and written once by every kernel here and go by the non-temporal way, which leaves the caches alone: unpermute of
+// 4096 x 4 rows of 2048 bf16 19.5 -> 16.8 us, of 16384 x 4 66 -> 58.5, permute of 8192 x 4 41 -> 35; the same for a handful of rows.  Vectors that every row needs, and
+// partial sums that the next launch reads, are cached.
+enum Caching { kStreamed, kCached };
+
+// elements 8 c .. 8 c + 7 of a row of K elements, zeros past its end; WHOLE: K is a multiple of eight (a kernel short of registers has both forms)
+template <typename T, bool WHOLE = false, int CACHING = kStreamed>
 __device__ __forceinline__ typename Piece<T>::raw load_piece(const T* row, int c, int K) {
   typename Piece<T>::raw v{};
-  if (8 * c + 8 <= K) {
-    v = *reinterpret_cast<const typename Piece<T>::mem*>(row + 8 * c);
+  if (WHOLE || 8 * c + 8 <= K) {
+    const auto* p = reinterpret_cast<const typename Piece<T>::mem*>(row + 8 * c);
+    if constexpr (CACHING == kStreamed) v = __builtin_nontemporal_load(p);
+    else v = *p;
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
@@ -54,10 +109,12 @@ __device__ __forceinline__ typename Piece<T>::raw load_piece(const T* row, int c
   }
   return v;
 }
-template <typename T>
+template <typename T, bool WHOLE = false, int CACHING = kStreamed>
 __device__ __forceinline__ void store_piece(T* row, int c, int K, typename Piece<T>::raw v) {
-  if (8 * c + 8 <= K) {
-    *reinterpret_cast<typename Piece<T>::mem*>(row + 8 * c) = v;
+  if (WHOLE || 8 * c + 8 <= K) {
+    auto* p = reinterpret_cast<typename Piece<T>::mem*>(row + 8 * c);
+    if constexpr (CACHING == kStreamed) __builtin_nontemporal_store(v, p);
+    else *p = v;
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
@@ -65,10 +122,11 @@ __device__ __forceinline__ void store_piece(T* row, int c, int K, typename Piece
   }
 }
 // the same of a vector whose type is known at run time only (norm weights: read once per workgroup, or from a cache)
+template <bool WHOLE = false>
 __device__ __forceinline__ f8 load_piece_of(int type, const void* row, int c, int K) {
-  if (type == kF32) return load_piece(reinterpret_cast<const float*>(row), c, K);
-  if (type == kF16) return Piece<_Float16>::widen(load_piece(reinterpret_cast<const _Float16*>(row), c, K));
-  return Piece<__bf16>::widen(load_piece(reinterpret_cast<const __bf16*>(row), c, K));
+  if (type == kF32) return Piece<float>::widen(load_piece<float, WHOLE, kCached>(reinterpret_cast<const float*>(row), c, K));
+  if (type == kF16) return Piece<_Float16>::widen(load_piece<_Float16, WHOLE, kCached>(reinterpret_cast<const _Float16*>(row), c, K));
+  return Piece<__bf16>::widen(load_piece<__bf16, WHOLE, kCached>(reinterpret_cast<const __bf16*>(row), c, K));
 }
 __device__ __forceinline__ float load_of(int type, const void* p, long i) {
   if (type == kF32) return reinterpret_cast<const float*>(p)[i];
@@ -97,26 +155,30 @@ __device__ __forceinline__ float wave_sum(float v) {
   return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
 }
 
-// Sums of N values each over the NT threads of a workgroup, in every thread.  One barrier: callers that sum again pass the other half of
-// their LDS (float [2][N * NT / 64]) in turn, so that no wave overwrites what another still reads.
+// Sums of N values each over the NT threads of a workgroup, in every thread.  Each wave leaves its N sums in LDS; behind the barrier lane W j + w of every wave reads the
+// sum that wave w has of value j, and groups of W lanes add up: some twelve instructions where every lane adding all of them takes N W.  One barrier: callers
+// that sum again pass the other half of their LDS (float [2][N * NT / 64]) in turn, so that no wave overwrites what another still reads.
 template <int NT, int N>
 __device__ __forceinline__ void group_sum(float (&v)[N], float* lds) {
 #pragma unroll
   for (int i = 0; i < N; ++i) v[i] = wave_sum(v[i]);
   if constexpr (NT > 64) {
-    constexpr int W = NT / 64;
-    const int wave = threadIdx.x >> 6;
-    if ((threadIdx.x & 63) == 0) {
+    constexpr int W = NT / 64, PER = 64 / W;  // waves (2, 4, 8 or 16); values whose sums one read brings
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    if (lane == 0) {
 #pragma unroll
       for (int i = 0; i < N; ++i) lds[i * W + wave] = v[i];
     }
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      float s = lds[i * W];
+    for (int i0 = 0; i0 < N; i0 += PER) {
+      float s = i0 * W + lane < N * W ? lds[i0 * W + lane] : 0.0f;
+      s = dpp_add<0x111, 0xF>(s);  // by 1, 2, 4, 8 lanes: lane i of a row of 16 ends with the sum of lanes i - W + 1 .. i
+      if constexpr (W >= 4) s = dpp_add<0x112, 0xF>(s);
+      if constexpr (W >= 8) s = dpp_add<0x114, 0xF>(s);
+      if constexpr (W >= 16) s = dpp_add<0x118, 0xF>(s);
 #pragma unroll
-      for (int w = 1; w < W; ++w) s += lds[i * W + w];
-      v[i] = s;
+      for (int i = i0; i < N && i < i0 + PER; ++i) v[i] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(s), (i - i0) * W + W - 1));
     }
   }
 }
