@@ -168,6 +168,15 @@ def current_stream() -> int:
     return _current_stream()
 
 
+def current_device() -> int:
+    """Index of torch's current device; as for the stream without the public call's checks (0.11 against 0.25 us) where torch has what is behind it."""
+    global current_device
+    import torch
+
+    current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+    return current_device()
+
+
 def check(lib: C.CDLL, rc: int) -> None:
     if rc != 0:
         raise RuntimeError(lib.mxmoe_last_error().decode())

@@ -25,44 +25,56 @@ _TYPES = {torch.float16: 0, torch.float32: 1, torch.bfloat16: 2}
 _NO_TYPE = "{} of dtype {}: fp16, fp32 or bf16 expected"
 
 
-def _call(dev: torch.device, name: str, *args) -> None:
-    """Entry point `name` on the current stream of `dev` (the library launches on the current device, whose stream it must be)."""
+def _call(index: int, name: str, *args) -> None:
+    """Entry point `name` on the current stream of GPU `index` (the library launches on the current device, whose stream it must be)."""
     lib = _lib.load()
-    if dev.index == torch.cuda.current_device():
+    if index == _lib.current_device():
         rc = getattr(lib, name)(*args, _lib.current_stream())
     else:
-        with torch.cuda.device(dev):
+        with torch.cuda.device(index):
             rc = getattr(lib, name)(*args, _lib.current_stream())
     if rc:
         _lib.check(lib, rc)
 
 
-def _rows(x: torch.Tensor, name: str, shape=None, dtype=None, dev=None) -> torch.Tensor:
-    """x as rows the kernels can read: 2-D, elements side by side (any row stride), a float type, on the GPU."""
-    if x.dim() != 2 or (shape is not None and tuple(x.shape) != shape):
+# (the checks of a call that has nothing wrong are one expression each: a decode step's operators are a few microseconds of host time)
+def _rows(x: torch.Tensor, name: str, shape=None, dtype=None, index=None) -> torch.Tensor:
+    """x as rows the kernels can read: 2-D, elements side by side (any row stride), a float type, on GPU `index` (None: any)."""
+    if (x.dim() == 2 and x.is_cuda and x.stride(1) == 1 and (x.dtype in _TYPES if dtype is None else x.dtype is dtype) and (shape is None or x.shape == shape)
+            and (index is None or x.get_device() == index)):
+        return x
+    if x.dim() != 2 or (shape is not None and x.shape != shape):
         raise ValueError(f"{name} of shape {list(x.shape)}: " + ("rows expected, [tokens, K]" if shape is None else f"{list(shape)} expected"))
     if x.dtype not in _TYPES or (dtype is not None and x.dtype != dtype):
         raise ValueError(_NO_TYPE.format(name, x.dtype) if dtype is None else f"{name} of dtype {x.dtype}: {dtype} expected")
-    _on(x, name, dev)
-    return x if x.stride(1) == 1 or x.shape[1] == 1 else x.contiguous()
+    _on(x, name, index)
+    return x if x.shape[1] == 1 else x.contiguous()
 
 
-def _on(x: torch.Tensor, name: str, dev) -> None:
-    if not x.is_cuda or (dev is not None and x.device != dev):
-        raise ValueError(f"{name} is on {x.device}: " + (f"{dev} expected" if dev is not None else "a GPU expected"))
+def _on(x: torch.Tensor, name: str, index) -> None:
+    if not x.is_cuda or (index is not None and x.get_device() != index):
+        raise ValueError(f"{name} is on {x.device}: " + (f"cuda:{index} expected" if index is not None else "a GPU expected"))
 
 
-def _output(out, shape, dtype, dev) -> torch.Tensor:
+def _output(out, like: torch.Tensor, rows: int, k: int, dtype) -> torch.Tensor:
+    """`out`, checked, or a new [rows, k] tensor of `dtype` on the device of `like`."""
     if out is None:
-        return torch.empty(shape, dtype=dtype, device=dev)
-    if tuple(out.shape) != tuple(shape) or out.dtype != dtype or out.device != dev or not out.is_contiguous():
-        raise ValueError(f"out: a contiguous tensor of shape {list(shape)} and dtype {dtype} on {dev} expected")
+        if like.dtype is dtype and like.shape[0] == rows and like.shape[1] == k and like.is_contiguous():
+            return torch.empty_like(like)
+        return torch.empty((rows, k), dtype=dtype, device=like.device)
+    if out.shape != (rows, k) or out.dtype != dtype or out.device != like.device or not out.is_contiguous():
+        raise ValueError(f"out: a contiguous tensor of shape {[rows, k]} and dtype {dtype} on {like.device} expected")
     return out
 
 
 def _recorded(*tensors, out=None) -> bool:
     """Whether autograd is to record a call with these inputs."""
-    if not torch.is_grad_enabled() or not any(isinstance(t, torch.Tensor) and t.requires_grad for t in tensors):
+    if not torch.is_grad_enabled():
+        return False
+    for t in tensors:
+        if t is not None and t.__class__ is not float and t.requires_grad:
+            break
+    else:
         return False
     if out is not None:
         raise ValueError("out= is for calls without gradients")
@@ -87,20 +99,20 @@ def permute_tokens(hidden: torch.Tensor, topk_ids: torch.Tensor, num_experts: in
 def _permute(hidden, topk_ids, num_experts, out, perm):
     x = _rows(hidden, "hidden")
     t, k = x.shape
-    dev = x.device
+    index = x.get_device()
     if topk_ids.dim() != 2 or topk_ids.shape[0] != t:
         raise ValueError(f"topk_ids of shape {list(topk_ids.shape)}: [{t}, top-k] expected")
-    if topk_ids.dtype != torch.int32 and topk_ids.dtype != torch.int64:
+    if topk_ids.dtype is not torch.int32 and topk_ids.dtype is not torch.int64:
         raise ValueError(f"topk_ids of dtype {topk_ids.dtype}: int32 or int64 expected")
-    _on(topk_ids, "topk_ids", dev)
+    _on(topk_ids, "topk_ids", index)
     ids = topk_ids.contiguous()
-    topk = ids.shape[1]
-    rows = _output(out, (t * topk, k), x.dtype, dev)
-    row_of_slot = torch.empty((t, topk), dtype=torch.int32, device=dev)
+    topk, wide, dev = ids.shape[1], ids.dtype is torch.int64, x.device
+    rows = _output(out, x, t * topk, k, x.dtype)
+    row_of_slot = torch.empty((t, topk), dtype=torch.int32, device=dev) if wide else torch.empty_like(ids)
     recv = torch.empty(max(num_experts, 0), dtype=torch.int64, device=dev)
-    need = _lib.load().mxmoe_permute_tokens_workspace_bytes(t, topk, num_experts)
+    need = _lib.load().mxmoe_permute_tokens_workspace_bytes(t, topk, num_experts) if t * topk > 4096 else 0
     ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    _call(dev, "mxmoe_permute_tokens", x.data_ptr(), x.stride(0), _TYPES[x.dtype], ids.data_ptr(), ids.element_size(), t, topk, num_experts, k, rows.data_ptr(), out is not None,
+    _call(index, "mxmoe_permute_tokens", x.data_ptr(), x.stride(0), _TYPES[x.dtype], ids.data_ptr(), 8 if wide else 4, t, topk, num_experts, k, rows.data_ptr(), out is not None,
           row_of_slot.data_ptr(), recv.data_ptr(), None if perm is None else perm.data_ptr(), None if ws is None else ws.data_ptr())
     return rows, row_of_slot, recv
 
@@ -116,23 +128,21 @@ def permute_with_indices(hidden, topk_ids, num_experts, perm):
 
 def permute_tokens_backward(grad_rows: torch.Tensor, row_of_slot: torch.Tensor) -> torch.Tensor:
     """Gradient of `permute_tokens`: grad_hidden[t] = sum of the gradients of token t's rows (fp32, in slot order, rounded once)."""
-    return unpermute_tokens(grad_rows.detach(), row_of_slot)
+    return _unpermute(grad_rows, row_of_slot, None, None, None)
 
 
-def _map(row_of_slot, dev):
-    if row_of_slot.dim() != 2 or row_of_slot.dtype != torch.int32:
+def _map(row_of_slot, index):
+    if row_of_slot.dim() != 2 or row_of_slot.dtype is not torch.int32:
         raise ValueError(f"row_of_slot: int32 [tokens, top-k] expected, got {row_of_slot.dtype} {list(row_of_slot.shape)}")
-    _on(row_of_slot, "row_of_slot", dev)
+    _on(row_of_slot, "row_of_slot", index)
     return row_of_slot.contiguous()
 
 
-def _weights(topk_weights, m, dev):
-    if topk_weights is None:
-        return None
+def _weights(topk_weights, m, index):
     if topk_weights.shape != m.shape:
         raise ValueError(f"topk_weights of shape {list(topk_weights.shape)}: {list(m.shape)} expected")
-    _on(topk_weights, "topk_weights", dev)
-    return topk_weights.to(torch.float32).contiguous()
+    _on(topk_weights, "topk_weights", index)
+    return (topk_weights if topk_weights.dtype is torch.float32 else topk_weights.to(torch.float32)).contiguous()
 
 
 def unpermute_tokens(rows: torch.Tensor, row_of_slot: torch.Tensor, topk_weights: torch.Tensor | None = None, shared: torch.Tensor | None = None,
@@ -141,14 +151,19 @@ def unpermute_tokens(rows: torch.Tensor, row_of_slot: torch.Tensor, topk_weights
     order, rounded once (for fp16 the bits of `gg_unpermute_out`).  A token none of whose slots names a row gets zeros (or its shared row).  Without weights all are 1."""
     if _recorded(rows, topk_weights, shared, out=out):
         return _Unpermute.apply(rows, row_of_slot, topk_weights, shared)
+    return _unpermute(rows, row_of_slot, topk_weights, shared, out)
+
+
+def _unpermute(rows, row_of_slot, topk_weights, shared, out):
     x = _rows(rows, "rows")
-    dev, k = x.device, x.shape[1]
-    m = _map(row_of_slot, dev)
-    w = _weights(topk_weights, m, dev)
+    index = x.get_device()
+    n, k = x.shape
+    m = _map(row_of_slot, index)
     t, topk = m.shape
-    sh = None if shared is None else _rows(shared, "shared", (t, k), x.dtype, dev)
-    y = _output(out, (t, k), x.dtype, dev)
-    _call(dev, "mxmoe_unpermute_tokens", x.data_ptr(), x.stride(0), x.shape[0], m.data_ptr(), None if w is None else w.data_ptr(), None if sh is None else sh.data_ptr(),
+    w = None if topk_weights is None else _weights(topk_weights, m, index)
+    sh = None if shared is None else _rows(shared, "shared", (t, k), x.dtype, index)
+    y = _output(out, x if sh is None else sh, t, k, x.dtype)
+    _call(index, "mxmoe_unpermute_tokens", x.data_ptr(), x.stride(0), n, m.data_ptr(), None if w is None else w.data_ptr(), None if sh is None else sh.data_ptr(),
           0 if sh is None else sh.stride(0), _TYPES[x.dtype], t, topk, k, y.data_ptr())
     return y
 
@@ -160,21 +175,22 @@ def unpermute_tokens_backward(grad_out: torch.Tensor, rows: torch.Tensor | None,
     grad_rows[row_of_slot[t, s]] = w[t, s] * grad_out[t]; rows that belong to dropped slots (those behind the last routed one, as `permute_tokens` numbers them) are zero,
     with `out` left as they were.  `rows` None (then `num_rows`, default T * k, says how many there are), or no weights: grad_weights is None."""
     g = _rows(grad_out, "grad_out")
-    dev, (t, k) = g.device, g.shape
-    m = _map(row_of_slot, dev)
+    index = g.get_device()
+    t, k = g.shape
+    m = _map(row_of_slot, index)
     if m.shape[0] != t:
         raise ValueError(f"row_of_slot of shape {list(m.shape)}: [{t}, top-k] expected")
-    w = _weights(topk_weights, m, dev)
     topk = m.shape[1]
+    w = None if topk_weights is None else _weights(topk_weights, m, index)
     x = None
     if rows is not None:
-        x = _rows(rows, "rows", (rows.shape[0], k), g.dtype, dev)
+        x = _rows(rows, "rows", (rows.shape[0], k), g.dtype, index)
         num_rows = x.shape[0]
     elif num_rows is None:
         num_rows = t * topk
-    grad_rows = _output(out, (num_rows, k), g.dtype, dev)
-    grad_w = torch.empty((t, topk), dtype=torch.float32, device=dev) if w is not None and x is not None else None
-    _call(dev, "mxmoe_unpermute_tokens_backward", g.data_ptr(), g.stride(0), None if x is None else x.data_ptr(), 0 if x is None else x.stride(0), num_rows, m.data_ptr(),
+    grad_rows = _output(out, g if x is None else x, num_rows, k, g.dtype)
+    grad_w = None if w is None or x is None else torch.empty_like(w)
+    _call(index, "mxmoe_unpermute_tokens_backward", g.data_ptr(), g.stride(0), None if x is None else x.data_ptr(), 0 if x is None else x.stride(0), num_rows, m.data_ptr(),
           None if w is None else w.data_ptr(), _TYPES[g.dtype], t, topk, k, grad_rows.data_ptr(), out is not None, None if grad_w is None else grad_w.data_ptr())
     return grad_rows, grad_w
 
@@ -184,60 +200,66 @@ def route_topk_backward(grad_weights: torch.Tensor, router_logits: torch.Tensor,
     if router_logits.dim() != 2 or router_logits.dtype not in _TYPES:
         raise ValueError(f"router logits of dtype {router_logits.dtype}, shape {list(router_logits.shape)}: fp16, fp32 or bf16 [tokens, experts] expected")
     _on(router_logits, "router_logits", None)
-    dev, (t, e) = router_logits.device, router_logits.shape
+    index, (t, e) = router_logits.get_device(), router_logits.shape
     if topk_ids.dim() != 2 or topk_ids.shape[0] != t or grad_weights.shape != topk_ids.shape:
         raise ValueError(f"topk_ids of shape {list(topk_ids.shape)}, grad_weights of shape {list(grad_weights.shape)}: [{t}, top-k] expected of both")
-    if topk_ids.dtype != torch.int32 and topk_ids.dtype != torch.int64:
+    if topk_ids.dtype is not torch.int32 and topk_ids.dtype is not torch.int64:
         raise ValueError(f"topk_ids of dtype {topk_ids.dtype}: int32 or int64 expected")
-    _on(topk_ids, "topk_ids", dev)
-    _on(grad_weights, "grad_weights", dev)
-    ids = topk_ids if topk_ids.dtype == torch.int32 else topk_ids.clamp(-1, e).to(torch.int32)
-    ids = ids.contiguous()
-    logits, g = router_logits.contiguous(), grad_weights.to(torch.float32).contiguous()
+    _on(topk_ids, "topk_ids", index)
+    ids = (topk_ids if topk_ids.dtype is torch.int32 else topk_ids.clamp(-1, e).to(torch.int32)).contiguous()
+    logits, g = router_logits.contiguous(), _weights(grad_weights, ids, index)
     out = torch.empty_like(logits)
-    _call(dev, "mxmoe_route_topk_backward", g.data_ptr(), logits.data_ptr(), _TYPES[logits.dtype], ids.data_ptr(), t, e, ids.shape[1], int(bool(renormalise)), out.data_ptr())
+    _call(index, "mxmoe_route_topk_backward", g.data_ptr(), logits.data_ptr(), _TYPES[logits.dtype], ids.data_ptr(), t, e, ids.shape[1], int(bool(renormalise)), out.data_ptr())
     return out
 
 
 # ---- norms, gate and residual scale ----
 
-def _vector(w, name, k, dtype, dev):
-    """(tensor or None, dtype of the vectors so far)."""
-    if w is None:
-        return None, dtype
-    if w.shape != (k,) or w.dtype not in _TYPES or (dtype is not None and w.dtype != dtype):
+def _vector(w, name, k, dtype, index):
+    """w [k] as the kernels can read it; `dtype`: that of the vectors before it, or None."""
+    if w.shape != (k,) or w.dtype not in _TYPES or (dtype is not None and w.dtype is not dtype):
         raise ValueError(f"{name} of dtype {w.dtype}, shape {list(w.shape)}: [{k}] in fp16, fp32 or bf16 expected, all vectors of one dtype")
-    _on(w, name, dev)
-    return w.contiguous(), w.dtype
+    _on(w, name, index)
+    return w.contiguous()
 
 
 def block_norm(x: torch.Tensor, weight: torch.Tensor | None = None, eps: float = 1e-6, out_dtype: torch.dtype | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
     """y = x / sqrt(mean(x^2) + eps) * weight over rows [T, K], in `out_dtype` (default x's): from a bfloat16 or fp32 residual stream into the fp16 layer in one pass."""
     if _recorded(x, weight, out=out):
         return _Norm.apply(x, weight, eps, out_dtype)
+    return _norm(x, weight, eps, out_dtype, out)
+
+
+def _norm(x, weight, eps, out_dtype, out):
     xr = _rows(x, "x")
-    dev, (t, k) = xr.device, xr.shape
-    w, wt = _vector(weight, "weight", k, None, dev)
-    od = xr.dtype if out_dtype is None else out_dtype
-    if od not in _TYPES:
-        raise ValueError(_NO_TYPE.format("output", od))
-    y = _output(out, (t, k), od, dev)
-    _call(dev, "mxmoe_block_norm", xr.data_ptr(), xr.stride(0), _TYPES[xr.dtype], None if w is None else w.data_ptr(), 1 if wt is None else _TYPES[wt], eps, t, k, y.data_ptr(), _TYPES[od])
+    index = xr.get_device()
+    t, k = xr.shape
+    w = None if weight is None else _vector(weight, "weight", k, None, index)
+    xt = _TYPES[xr.dtype]
+    if out_dtype is None:
+        out_dtype = xr.dtype
+    elif out_dtype not in _TYPES:
+        raise ValueError(_NO_TYPE.format("output", out_dtype))
+    y = _output(out, xr, t, k, out_dtype)
+    _call(index, "mxmoe_block_norm", xr.data_ptr(), xr.stride(0), xt, None if w is None else w.data_ptr(), 1 if w is None else _TYPES[w.dtype], eps, t, k, y.data_ptr(), _TYPES[out_dtype])
     return y
 
 
 def block_norm_backward(grad_y: torch.Tensor, x: torch.Tensor, weight: torch.Tensor | None = None, eps: float = 1e-6, grad_residual: torch.Tensor | None = None):
     """Gradients of `block_norm` -> (grad_x, grad_weight or None).  `grad_residual` [T, K] (x's dtype), the gradient that reaches x past the norm, is added to grad_x."""
     xr = _rows(x, "x")
-    dev, (t, k) = xr.device, xr.shape
-    gy = _rows(grad_y, "grad_y", (t, k), None, dev)
-    gr = None if grad_residual is None else _rows(grad_residual, "grad_residual", (t, k), xr.dtype, dev)
-    w, wt = _vector(weight, "weight", k, None, dev)
-    grad_x = torch.empty((t, k), dtype=xr.dtype, device=dev)
-    grad_w, ws = (None, None) if w is None else (torch.empty_like(w), _workspace(t, k, dev))
-    _call(dev, "mxmoe_block_norm_backward", gy.data_ptr(), gy.stride(0), _TYPES[gy.dtype], xr.data_ptr(), xr.stride(0), _TYPES[xr.dtype], None if w is None else w.data_ptr(),
-          1 if wt is None else _TYPES[wt], None if gr is None else gr.data_ptr(), 0 if gr is None else gr.stride(0), eps, t, k, grad_x.data_ptr(), None if w is None else grad_w.data_ptr(),
-          None if ws is None else ws.data_ptr())
+    index = xr.get_device()
+    t, k = xr.shape
+    gy = _rows(grad_y, "grad_y", (t, k), None, index)
+    gr = None if grad_residual is None else _rows(grad_residual, "grad_residual", (t, k), xr.dtype, index)
+    grad_x = _output(None, xr, t, k, xr.dtype)
+    w = grad_w = ws = None
+    if weight is not None:
+        w = _vector(weight, "weight", k, None, index)
+        grad_w, ws = torch.empty_like(w), _workspace(t, k, xr.device)
+    _call(index, "mxmoe_block_norm_backward", gy.data_ptr(), gy.stride(0), _TYPES[gy.dtype], xr.data_ptr(), xr.stride(0), _TYPES[xr.dtype], None if w is None else w.data_ptr(),
+          1 if w is None else _TYPES[w.dtype], None if gr is None else gr.data_ptr(), 0 if gr is None else gr.stride(0), eps, t, k, grad_x.data_ptr(),
+          None if w is None else grad_w.data_ptr(), None if ws is None else ws.data_ptr())
     return grad_x, grad_w
 
 
@@ -245,9 +267,9 @@ def _workspace(t, k, dev):
     return torch.empty(_lib.load().mxmoe_block_backward_workspace_bytes(t, k), dtype=torch.uint8, device=dev)
 
 
-def _gate(gate, gate_act, z, dev):
+def _gate(gate, gate_act, z, index):
     """(kind, tensor or None, stride, dtype, sigmoid)."""
-    if gate_act not in (None, "sigmoid"):
+    if gate_act is not None and gate_act != "sigmoid":
         raise ValueError(f"gate_act {gate_act!r}: None or 'sigmoid' expected")
     if gate is None:
         return 0, None, 0, 1, 0
@@ -255,30 +277,37 @@ def _gate(gate, gate_act, z, dev):
     if gate.shape == (t,) or gate.shape == (t, 1):
         if gate.dtype not in _TYPES:
             raise ValueError(_NO_TYPE.format("gate", gate.dtype))
-        _on(gate, "gate", dev)
+        _on(gate, "gate", index)
         return 1, gate, gate.stride(0), _TYPES[gate.dtype], int(gate_act is not None)
     if gate.shape != (t, k):
         raise ValueError(f"gate of shape {list(gate.shape)}: [{t}], [{t}, 1] or [{t}, {k}] expected")
-    gate = _rows(gate, "gate", (t, k), z.dtype, dev)
+    gate = _rows(gate, "gate", (t, k), z.dtype, index)
     return 2, gate, gate.stride(0), _TYPES[gate.dtype], int(gate_act is not None)
 
 
 def _residual_inputs(x, z, gate, gate_act, scale, norm_weight, next_weight):
+    """(arguments of the entry points, the tensors behind them)."""
     xr = _rows(x, "x")
-    dev, (t, k) = xr.device, xr.shape
-    zr = _rows(z, "z", (t, k), None, dev)
-    kind, g, ldg, gt, sigmoid = _gate(gate, gate_act, zr, dev)
-    factor, vec = 1.0, None
-    if isinstance(scale, torch.Tensor):
-        vec = scale
-    elif scale is not None:
-        factor = float(scale)
-    vec, wt = _vector(vec, "scale", k, None, dev)
-    w1, wt = _vector(norm_weight, "norm_weight", k, wt, dev)
-    w2, wt = _vector(next_weight, "next_weight", k, wt, dev)
+    index = xr.get_device()
+    t, k = xr.shape
+    zr = _rows(z, "z", (t, k), None, index)
+    kind, g, ldg, gt, sigmoid = _gate(gate, gate_act, zr, index)
+    factor, vec, w1, w2, wt = 1.0, None, None, None, None
+    if scale is not None:
+        if isinstance(scale, torch.Tensor):
+            vec = _vector(scale, "scale", k, None, index)
+            wt = vec.dtype
+        else:
+            factor = float(scale)
+    if norm_weight is not None:
+        w1 = _vector(norm_weight, "norm_weight", k, wt, index)
+        wt = w1.dtype
+    if next_weight is not None:
+        w2 = _vector(next_weight, "next_weight", k, wt, index)
+        wt = w2.dtype
     args = (xr.data_ptr(), xr.stride(0), _TYPES[xr.dtype], zr.data_ptr(), zr.stride(0), _TYPES[zr.dtype], kind, None if g is None else g.data_ptr(), ldg, gt, sigmoid, factor,
             None if vec is None else vec.data_ptr(), None if w1 is None else w1.data_ptr(), None if w2 is None else w2.data_ptr(), 1 if wt is None else _TYPES[wt])
-    return args, (xr, zr, g, vec, w1, w2)
+    return args, xr, zr, g, vec, w1, w2
 
 
 def block_residual(x: torch.Tensor, z: torch.Tensor, *, gate: torch.Tensor | None = None, gate_act: str | None = None, scale: float | torch.Tensor | None = None,
@@ -293,13 +322,17 @@ def block_residual(x: torch.Tensor, z: torch.Tensor, *, gate: torch.Tensor | Non
         vec, factor = (scale, None) if isinstance(scale, torch.Tensor) else (None, scale)
         h, y = _Residual.apply(x, z, gate, vec, norm_weight, next_weight, gate_act, factor, eps)
         return h if next_weight is None else (h, y)
-    args, (xr, zr, *keep) = _residual_inputs(x, z, gate, gate_act, scale, norm_weight, next_weight)
+    return _residual(x, z, gate, gate_act, scale, norm_weight, next_weight, eps, out)
+
+
+def _residual(x, z, gate, gate_act, scale, norm_weight, next_weight, eps, out):
+    args, xr, zr, g, vec, w1, w2 = _residual_inputs(x, z, gate, gate_act, scale, norm_weight, next_weight)
     t, k = xr.shape
     if out is not None and xr is not x and out.data_ptr() == x.data_ptr():
         raise ValueError("out may be x only where x's elements lie side by side")
-    h = _output(out, (t, k), xr.dtype, xr.device)
-    y = None if next_weight is None else torch.empty((t, k), dtype=zr.dtype, device=xr.device)
-    _call(xr.device, "mxmoe_block_residual", *args, eps, t, k, h.data_ptr(), None if y is None else y.data_ptr())
+    h = _output(out, xr, t, k, xr.dtype)
+    y = None if w2 is None else _output(None, zr, t, k, zr.dtype)
+    _call(xr.get_device(), "mxmoe_block_residual", *args, eps, t, k, h.data_ptr(), None if y is None else y.data_ptr())
     return h if y is None else (h, y)
 
 
@@ -307,22 +340,23 @@ def block_residual_backward(grad_h: torch.Tensor | None, grad_y: torch.Tensor | 
                             scale: float | torch.Tensor | None = None, norm_weight: torch.Tensor | None = None, next_weight: torch.Tensor | None = None, eps: float = 1e-6):
     """Gradients of `block_residual` -> (grad_x, grad_z, grad_gate, grad_scale, grad_norm_weight, grad_next_weight), None for inputs that were not given or are numbers.
     grad_h (x's dtype) or grad_y (z's dtype) may be None.  Nothing is kept from the forward call."""
-    args, (xr, zr, g, vec, w1, w2) = _residual_inputs(x, z, gate, gate_act, scale, norm_weight, next_weight)
-    dev, (t, k) = xr.device, xr.shape
-    if grad_y is not None and next_weight is None:
+    args, xr, zr, g, vec, w1, w2 = _residual_inputs(x, z, gate, gate_act, scale, norm_weight, next_weight)
+    index = xr.get_device()
+    t, k = xr.shape
+    if grad_y is not None and w2 is None:
         raise ValueError("grad_y without next_weight: the call had no y")
     if grad_h is None and grad_y is None:
         raise ValueError("neither grad_h nor grad_y is given")
-    gh = None if grad_h is None else _rows(grad_h, "grad_h", (t, k), xr.dtype, dev)
-    gy = None if grad_y is None else _rows(grad_y, "grad_y", (t, k), zr.dtype, dev)
-    grad_x, grad_z = torch.empty((t, k), dtype=xr.dtype, device=dev), torch.empty((t, k), dtype=zr.dtype, device=dev)
-    grad_gate = None if g is None else torch.empty(gate.shape, dtype=gate.dtype, device=dev)
-    grads = [None if w is None else torch.empty_like(w) for w in (vec, w1, w2)]
-    ws = None if all(w is None for w in grads) else _workspace(t, k, dev)
-    ptr = [None if w is None else w.data_ptr() for w in (gh, gy, grad_gate, *grads, ws)]
-    _call(dev, "mxmoe_block_residual_backward", ptr[0], 0 if gh is None else gh.stride(0), ptr[1], 0 if gy is None else gy.stride(0), *args, eps, t, k, grad_x.data_ptr(),
-          grad_z.data_ptr(), *ptr[2:])
-    return grad_x, grad_z, grad_gate, *grads
+    gh = None if grad_h is None else _rows(grad_h, "grad_h", (t, k), xr.dtype, index)
+    gy = None if grad_y is None else _rows(grad_y, "grad_y", (t, k), zr.dtype, index)
+    grad_x, grad_z = _output(None, xr, t, k, xr.dtype), _output(None, zr, t, k, zr.dtype)
+    grad_gate = None if g is None else torch.empty(gate.shape, dtype=gate.dtype, device=gate.device)
+    grad_s, grad_1, grad_2 = (None if w is None else torch.empty_like(w) for w in (vec, w1, w2))
+    ws = None if vec is None and w1 is None and w2 is None else _workspace(t, k, xr.device)
+    _call(index, "mxmoe_block_residual_backward", None if gh is None else gh.data_ptr(), 0 if gh is None else gh.stride(0), None if gy is None else gy.data_ptr(),
+          0 if gy is None else gy.stride(0), *args, eps, t, k, grad_x.data_ptr(), grad_z.data_ptr(), None if grad_gate is None else grad_gate.data_ptr(),
+          None if grad_s is None else grad_s.data_ptr(), None if grad_1 is None else grad_1.data_ptr(), None if grad_2 is None else grad_2.data_ptr(), None if ws is None else ws.data_ptr())
+    return grad_x, grad_z, grad_gate, grad_s, grad_1, grad_2
 
 
 # ---- the same for autograd ----
