@@ -25,6 +25,17 @@ _TYPES = {torch.float16: 0, torch.float32: 1, torch.bfloat16: 2}
 _NO_TYPE = "{} of dtype {}: fp16, fp32 or bf16 expected"
 
 
+_fast = None
+
+
+def _calls():
+    """The native form of the calls in which nothing has to be copied, recorded or refused (csrc/block_calls.cpp); its functions return None for all others."""
+    global _fast
+    if _fast is None:
+        _fast = _lib.block_calls()
+    return _fast
+
+
 def _call(index: int, name: str, *args) -> None:
     """Entry point `name` on the current stream of GPU `index` (the library launches on the current device, whose stream it must be)."""
     lib = _lib.load()
@@ -72,7 +83,7 @@ def _recorded(*tensors, out=None) -> bool:
     if not torch.is_grad_enabled():
         return False
     for t in tensors:
-        if t is not None and t.__class__ is not float and t.requires_grad:
+        if isinstance(t, torch.Tensor) and t.requires_grad:
             break
     else:
         return False
@@ -91,6 +102,10 @@ def permute_tokens(hidden: torch.Tensor, topk_ids: torch.Tensor, num_experts: in
     Stable order by (expert, flattened (token, slot)), as `build_permutation`.  Ids (int32 or int64) outside [0, E), such as -1 for padding tokens or for experts of
     another GPU, name no expert: their rows come behind all others and are zero, and row_of_slot holds -2 - row for them.  With `out` [T * k, K] the rows go there,
     and those behind the last routed one are left as they were."""
+    if out is None:
+        got = (_fast or _calls()).permute_tokens(hidden, topk_ids, num_experts)
+        if got is not None:
+            return got
     if _recorded(hidden, out=out):
         return _Permute.apply(hidden, topk_ids, num_experts, None)
     return _permute(hidden, topk_ids, num_experts, out, None)
@@ -128,7 +143,8 @@ def permute_with_indices(hidden, topk_ids, num_experts, perm):
 
 def permute_tokens_backward(grad_rows: torch.Tensor, row_of_slot: torch.Tensor) -> torch.Tensor:
     """Gradient of `permute_tokens`: grad_hidden[t] = sum of the gradients of token t's rows (fp32, in slot order, rounded once)."""
-    return _unpermute(grad_rows, row_of_slot, None, None, None)
+    got = (_fast or _calls()).unpermute_tokens(grad_rows.detach(), row_of_slot, None, None)
+    return got if got is not None else _unpermute(grad_rows, row_of_slot, None, None, None)
 
 
 def _map(row_of_slot, index):
@@ -149,6 +165,10 @@ def unpermute_tokens(rows: torch.Tensor, row_of_slot: torch.Tensor, topk_weights
                      out: torch.Tensor | None = None) -> torch.Tensor:
     """Sorted rows back in token order: out[t] = sum_s topk_weights[t, s] * rows[row_of_slot[t, s]] (+ shared[t]), slots with a negative entry left out; fp32 in slot
     order, rounded once (for fp16 the bits of `gg_unpermute_out`).  A token none of whose slots names a row gets zeros (or its shared row).  Without weights all are 1."""
+    if out is None:
+        got = (_fast or _calls()).unpermute_tokens(rows, row_of_slot, topk_weights, shared)
+        if got is not None:
+            return got
     if _recorded(rows, topk_weights, shared, out=out):
         return _Unpermute.apply(rows, row_of_slot, topk_weights, shared)
     return _unpermute(rows, row_of_slot, topk_weights, shared, out)
@@ -174,6 +194,10 @@ def unpermute_tokens_backward(grad_out: torch.Tensor, rows: torch.Tensor | None,
 
     grad_rows[row_of_slot[t, s]] = w[t, s] * grad_out[t]; rows that belong to dropped slots (those behind the last routed one, as `permute_tokens` numbers them) are zero,
     with `out` left as they were.  `rows` None (then `num_rows`, default T * k, says how many there are), or no weights: grad_weights is None."""
+    if out is None:
+        got = (_fast or _calls()).unpermute_tokens_backward(grad_out, rows, row_of_slot, topk_weights)
+        if got is not None:
+            return got
     g = _rows(grad_out, "grad_out")
     index = g.get_device()
     t, k = g.shape
@@ -197,6 +221,9 @@ def unpermute_tokens_backward(grad_out: torch.Tensor, rows: torch.Tensor | None,
 
 def route_topk_backward(grad_weights: torch.Tensor, router_logits: torch.Tensor, topk_ids: torch.Tensor, renormalise: bool = False) -> torch.Tensor:
     """Gradient of `route_topk`'s weights [T, k] with respect to its logits [T, E], in the logits' dtype, for the experts that it chose (`topk_ids` int32 or int64 [T, k])."""
+    got = (_fast or _calls()).route_topk_backward(grad_weights, router_logits, topk_ids, renormalise)
+    if got is not None:
+        return got
     if router_logits.dim() != 2 or router_logits.dtype not in _TYPES:
         raise ValueError(f"router logits of dtype {router_logits.dtype}, shape {list(router_logits.shape)}: fp16, fp32 or bf16 [tokens, experts] expected")
     _on(router_logits, "router_logits", None)
@@ -225,6 +252,10 @@ def _vector(w, name, k, dtype, index):
 
 def block_norm(x: torch.Tensor, weight: torch.Tensor | None = None, eps: float = 1e-6, out_dtype: torch.dtype | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
     """y = x / sqrt(mean(x^2) + eps) * weight over rows [T, K], in `out_dtype` (default x's): from a bfloat16 or fp32 residual stream into the fp16 layer in one pass."""
+    if out is None:
+        y = (_fast or _calls()).block_norm(x, weight, eps, out_dtype)
+        if y is not None:
+            return y
     if _recorded(x, weight, out=out):
         return _Norm.apply(x, weight, eps, out_dtype)
     return _norm(x, weight, eps, out_dtype, out)
@@ -247,6 +278,9 @@ def _norm(x, weight, eps, out_dtype, out):
 
 def block_norm_backward(grad_y: torch.Tensor, x: torch.Tensor, weight: torch.Tensor | None = None, eps: float = 1e-6, grad_residual: torch.Tensor | None = None):
     """Gradients of `block_norm` -> (grad_x, grad_weight or None).  `grad_residual` [T, K] (x's dtype), the gradient that reaches x past the norm, is added to grad_x."""
+    got = (_fast or _calls()).block_norm_backward(grad_y, x, weight, eps, grad_residual)
+    if got is not None:
+        return got
     xr = _rows(x, "x")
     index = xr.get_device()
     t, k = xr.shape
@@ -318,6 +352,10 @@ def block_residual(x: torch.Tensor, z: torch.Tensor, *, gate: torch.Tensor | Non
     norm(z) = z / sqrt(mean(z^2) + eps) * norm_weight, or z itself without `norm_weight`.  `gate` per token ([T] or [T, 1]) or per element ([T, K], z's dtype), through a
     sigmoid with gate_act="sigmoid" (a shared expert's gate, say).  `scale`: a number, or one per channel [K].  The vectors have one dtype.  Everything is fp32 inside; y
     is computed from h before its rounding.  `out` (x itself is allowed) receives h."""
+    if out is None:
+        got = (_fast or _calls()).block_residual(x, z, gate, gate_act, scale, norm_weight, next_weight, eps)
+        if got is not None:
+            return got
     if _recorded(x, z, gate, scale, norm_weight, next_weight, out=out):
         vec, factor = (scale, None) if isinstance(scale, torch.Tensor) else (None, scale)
         h, y = _Residual.apply(x, z, gate, vec, norm_weight, next_weight, gate_act, factor, eps)
@@ -340,6 +378,9 @@ def block_residual_backward(grad_h: torch.Tensor | None, grad_y: torch.Tensor | 
                             scale: float | torch.Tensor | None = None, norm_weight: torch.Tensor | None = None, next_weight: torch.Tensor | None = None, eps: float = 1e-6):
     """Gradients of `block_residual` -> (grad_x, grad_z, grad_gate, grad_scale, grad_norm_weight, grad_next_weight), None for inputs that were not given or are numbers.
     grad_h (x's dtype) or grad_y (z's dtype) may be None.  Nothing is kept from the forward call."""
+    got = (_fast or _calls()).block_residual_backward(grad_h, grad_y, x, z, gate, gate_act, scale, norm_weight, next_weight, eps)
+    if got is not None:
+        return got
     args, xr, zr, g, vec, w1, w2 = _residual_inputs(x, z, gate, gate_act, scale, norm_weight, next_weight)
     index = xr.get_device()
     t, k = xr.shape

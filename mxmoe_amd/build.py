@@ -14,6 +14,7 @@ from pathlib import Path
 PKG = Path(__file__).resolve().parent
 CSRC = PKG / "csrc"
 LIB = PKG / "libmxmoe_amd.so"
+CALLS = PKG / "_block_calls.so"
 
 HIPCC_FLAGS = [
     "--offload-arch=gfx950",
@@ -216,6 +217,23 @@ def hipcc_build(sources, out: Path, extra=(), verbose: bool = False, jobs: int =
     return out
 
 
+def build_calls() -> Path:
+    """Compile the host-side extension of `mxmoe_amd.block` (csrc/block_calls.cpp: no device code, torch's own headers) with the host compiler."""
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+
+    inc = [f"-I{p}" for p in (*cpp_extension.include_paths(), sysconfig.get_paths()["include"])]
+    lib = Path(torch.__file__).parent / "lib"
+    cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *inc, str(CSRC / "block_calls.cpp"),
+           "-o", str(CALLS), f"-L{lib}", "-ltorch_python", "-ltorch_cpu", "-lc10"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"g++ failed ({res.returncode}):\n{' '.join(cmd)}\n{res.stderr}")
+    return CALLS
+
+
 def build_default(verbose: bool = False) -> Path:
     """Compile every .hip translation unit of the package, and the generator's registration unit of the default kernels, into
     libmxmoe_amd.so."""
@@ -248,5 +266,6 @@ def build_generated_sample(verbose: bool = False) -> Path:
 
 
 if __name__ == "__main__":
+    print(build_calls())
     print(build_default(verbose=True))
     print(build_generated_sample(verbose=True))

@@ -1,0 +1,343 @@
+// The host side of the operators of mxmoe_amd/block.py for calls in which nothing has to be copied, recorded or refused: tensors are looked at, outputs allocated and the C
+// entry point is called without going through Python for each.  A call of block.py costs 3 - 15 us of host time in Python beside the 3 us that a launch takes, more than
+// the GPU needs for a decode step's rows.
+//
+// Every function takes its operator's arguments in order and returns its results, or None where the call is not of that kind: then block.py does it, with the checks
+// that say what is wrong.  It has no rules of its own: what it takes is a part of what block.py takes, with the same results.
+#include <ATen/ATen.h>
+#include <c10/core/GradMode.h>
+#include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/Dtype.h>
+
+#include <cstdint>
+#include <cstring>
+
+#include "../../include/mxmoe_amd.h"
+
+namespace {
+
+// entry points of the library and torch's functions for the current device and stream, given by bind()
+struct Library {
+  decltype(&mxmoe_last_error) last_error;
+  decltype(&mxmoe_permute_tokens_workspace_bytes) permute_workspace;
+  decltype(&mxmoe_permute_tokens) permute;
+  decltype(&mxmoe_unpermute_tokens) unpermute;
+  decltype(&mxmoe_unpermute_tokens_backward) unpermute_backward;
+  decltype(&mxmoe_route_topk_backward) route_backward;
+  decltype(&mxmoe_block_norm) norm;
+  decltype(&mxmoe_block_residual) residual;
+  decltype(&mxmoe_block_backward_workspace_bytes) backward_workspace;
+  decltype(&mxmoe_block_norm_backward) norm_backward;
+  decltype(&mxmoe_block_residual_backward) residual_backward;
+} lib{};
+PyObject* get_device = nullptr;
+PyObject* get_stream = nullptr;
+
+const at::Tensor kNone;
+
+// An argument as a tensor; `ok` falls where it is something else.  None is an undefined tensor.
+const at::Tensor& tensor(PyObject* o, bool& ok) {
+  if (o == Py_None) return kNone;
+  if (!THPVariable_CheckExact(o)) {
+    ok = false;
+    return kNone;
+  }
+  return THPVariable_Unpack(o);
+}
+int float_type(const at::Tensor& t) {
+  switch (t.scalar_type()) {
+    case at::kHalf: return 0;
+    case at::kFloat: return 1;
+    case at::kBFloat16: return 2;
+    default: return -1;
+  }
+}
+bool on(const at::Tensor& t, int device) { return t.is_cuda() && t.get_device() == device; }
+bool rows(const at::Tensor& t, int device) { return t.dim() == 2 && on(t, device) && t.stride(1) == 1 && float_type(t) >= 0; }
+bool rows(const at::Tensor& t, int device, int64_t n, int64_t k) { return rows(t, device) && t.size(0) == n && t.size(1) == k; }
+bool vector(const at::Tensor& t, int device, int64_t k) { return t.dim() == 1 && t.size(0) == k && on(t, device) && t.is_contiguous() && float_type(t) >= 0; }
+void* ptr(const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+int64_t ld(const at::Tensor& t) { return t.defined() ? t.stride(0) : 0; }
+constexpr int64_t kMost = 1 << 30;  // sizes past what an entry point's int holds go the long way
+
+bool wants_grad(std::initializer_list<const at::Tensor*> ts) {
+  if (!c10::GradMode::is_enabled()) return false;
+  for (const at::Tensor* t : ts)
+    if (t->defined() && t->requires_grad()) return true;
+  return false;
+}
+// Current device (-1 where torch cannot say) and its current stream
+int current_device() {
+  PyObject* d = PyObject_CallNoArgs(get_device);
+  if (!d) throw python_error();
+  const long v = PyLong_AsLong(d);
+  Py_DECREF(d);
+  return (int)v;
+}
+void* current_stream(int device) {
+  PyObject* i = PyLong_FromLong(device);
+  PyObject* s = PyObject_CallOneArg(get_stream, i);
+  Py_XDECREF(i);
+  if (!s) throw python_error();
+  void* v = PyLong_AsVoidPtr(s);
+  Py_DECREF(s);
+  return v;
+}
+at::Tensor rows_like(const at::Tensor& t, int64_t n, int64_t k, at::ScalarType type) { return at::empty({n, k}, t.options().dtype(type).requires_grad(false)); }
+at::Tensor bytes(const at::Tensor& t, size_t n) { return at::empty({(int64_t)n}, t.options().dtype(at::kByte).requires_grad(false)); }
+
+PyObject* wrap(const at::Tensor& t) {
+  if (!t.defined()) Py_RETURN_NONE;
+  return THPVariable_Wrap(t);
+}
+template <typename... T>
+PyObject* tuple(const T&... t) {
+  PyObject* r = PyTuple_New(sizeof...(t));
+  if (!r) throw python_error();
+  Py_ssize_t i = 0;
+  for (PyObject* o : {wrap(t)...}) PyTuple_SET_ITEM(r, i++, o);
+  return r;
+}
+PyObject* failed() {
+  PyErr_SetString(PyExc_RuntimeError, lib.last_error());
+  return nullptr;
+}
+bool truth(PyObject* o) {
+  const int v = PyObject_IsTrue(o);
+  if (v < 0) throw python_error();
+  return v;
+}
+double number(PyObject* o) {
+  const double v = PyFloat_AsDouble(o);
+  if (v == -1.0 && PyErr_Occurred()) throw python_error();
+  return v;
+}
+
+#define NOT_MINE Py_RETURN_NONE
+#define ARGS(N) \
+  HANDLE_TH_ERRORS \
+  if (n_args != N || !lib.norm) NOT_MINE; \
+  [[maybe_unused]] bool ok = true
+
+// hidden, topk_ids, num_experts
+PyObject* permute_tokens(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
+  ARGS(3);
+  const at::Tensor &x = tensor(args[0], ok), &ids = tensor(args[1], ok);
+  if (!ok || !x.defined() || !ids.defined() || !PyLong_CheckExact(args[2])) NOT_MINE;
+  if (!x.is_cuda()) NOT_MINE;
+  const int device = current_device();
+  const long experts = PyLong_AsLong(args[2]);
+  if (!rows(x, device) || wants_grad({&x}) || ids.dim() != 2 || !on(ids, device) || !ids.is_contiguous() || ids.size(0) != x.size(0) || x.size(0) * ids.size(1) > kMost || x.size(1) > kMost ||
+      experts < 0 || experts > 4096 || (ids.scalar_type() != at::kInt && ids.scalar_type() != at::kLong))
+    NOT_MINE;
+  const int64_t t = x.size(0), k = ids.size(1), w = x.size(1);
+  at::Tensor out = rows_like(x, t * k, w, x.scalar_type()), map = rows_like(ids, t, k, at::kInt), recv = at::empty({experts}, ids.options().dtype(at::kLong)), ws;
+  if (const size_t need = lib.permute_workspace((int)t, (int)k, (int)experts)) ws = bytes(x, need);
+  if (lib.permute(ptr(x), x.stride(0), float_type(x), ptr(ids), (int)ids.element_size(), (int)t, (int)k, (int)experts, (int)w, ptr(out), 0, (int32_t*)ptr(map), (int64_t*)ptr(recv), nullptr, ptr(ws),
+                  current_stream(device)))
+    return failed();
+  return tuple(out, map, recv);
+  END_HANDLE_TH_ERRORS
+}
+
+bool slot_map(const at::Tensor& m, int device) { return m.defined() && m.dim() == 2 && m.scalar_type() == at::kInt && on(m, device) && m.is_contiguous() && m.numel() <= kMost; }
+bool weights_of(const at::Tensor& w, const at::Tensor& m, int device) {
+  return !w.defined() || (w.scalar_type() == at::kFloat && on(w, device) && w.is_contiguous() && w.sizes() == m.sizes());
+}
+
+// rows, row_of_slot, topk_weights, shared
+PyObject* unpermute_tokens(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
+  ARGS(4);
+  const at::Tensor &x = tensor(args[0], ok), &m = tensor(args[1], ok), &w = tensor(args[2], ok), &shared = tensor(args[3], ok);
+  if (!ok || !x.defined() || !x.is_cuda()) NOT_MINE;
+  const int device = current_device();
+  if (!rows(x, device) || !slot_map(m, device) || !weights_of(w, m, device) || wants_grad({&x, &w, &shared}) || x.size(0) > kMost || x.size(1) > kMost) NOT_MINE;
+  const int64_t t = m.size(0), k = m.size(1), width = x.size(1);
+  if (shared.defined() && (!rows(shared, device, t, width) || shared.scalar_type() != x.scalar_type())) NOT_MINE;
+  at::Tensor out = rows_like(x, t, width, x.scalar_type());
+  if (lib.unpermute(ptr(x), x.stride(0), (int)x.size(0), (const int32_t*)ptr(m), (const float*)ptr(w), ptr(shared), ld(shared), float_type(x), (int)t, (int)k, (int)width, ptr(out),
+                    current_stream(device)))
+    return failed();
+  return wrap(out);
+  END_HANDLE_TH_ERRORS
+}
+
+// grad_out, rows, row_of_slot, topk_weights (both given)
+PyObject* unpermute_tokens_backward(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
+  ARGS(4);
+  const at::Tensor &g = tensor(args[0], ok), &x = tensor(args[1], ok), &m = tensor(args[2], ok), &w = tensor(args[3], ok);
+  if (!ok || !g.defined() || !x.defined() || !w.defined() || !x.is_cuda()) NOT_MINE;
+  const int device = current_device();
+  if (!rows(g, device) || !rows(x, device) || x.size(1) != g.size(1) || x.scalar_type() != g.scalar_type() || !slot_map(m, device) || m.size(0) != g.size(0) || !weights_of(w, m, device) ||
+      x.size(0) > kMost || x.size(1) > kMost)
+    NOT_MINE;
+  at::Tensor grad_rows = rows_like(x, x.size(0), x.size(1), x.scalar_type()), grad_weights = rows_like(w, m.size(0), m.size(1), at::kFloat);
+  if (lib.unpermute_backward(ptr(g), g.stride(0), ptr(x), x.stride(0), (int)x.size(0), (const int32_t*)ptr(m), (const float*)ptr(w), float_type(x), (int)m.size(0), (int)m.size(1), (int)x.size(1),
+                             ptr(grad_rows), 0, (float*)ptr(grad_weights), current_stream(device)))
+    return failed();
+  return tuple(grad_rows, grad_weights);
+  END_HANDLE_TH_ERRORS
+}
+
+// grad_weights, router_logits, topk_ids, renormalise
+PyObject* route_topk_backward(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
+  ARGS(4);
+  const at::Tensor &g = tensor(args[0], ok), &x = tensor(args[1], ok), &ids = tensor(args[2], ok);
+  if (!ok || !g.defined() || !x.defined() || !ids.defined() || !x.is_cuda()) NOT_MINE;
+  const int device = current_device();
+  if (!rows(x, device) || !x.is_contiguous() || !slot_map(ids, device) || ids.size(0) != x.size(0) || !weights_of(g, ids, device) || x.size(0) > kMost || x.size(1) > kMost) NOT_MINE;
+  at::Tensor out = rows_like(x, x.size(0), x.size(1), x.scalar_type());
+  if (lib.route_backward((const float*)ptr(g), ptr(x), float_type(x), (const int32_t*)ptr(ids), (int)x.size(0), (int)x.size(1), (int)ids.size(1), truth(args[3]), ptr(out), current_stream(device)))
+    return failed();
+  return wrap(out);
+  END_HANDLE_TH_ERRORS
+}
+
+// x, weight, eps, out_dtype
+PyObject* block_norm(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
+  ARGS(4);
+  const at::Tensor &x = tensor(args[0], ok), &w = tensor(args[1], ok);
+  if (!ok || !x.defined() || !x.is_cuda() || !(args[3] == Py_None || THPDtype_Check(args[3]))) NOT_MINE;
+  const int device = current_device();
+  if (!rows(x, device) || (w.defined() && !vector(w, device, x.size(1))) || wants_grad({&x, &w}) || x.size(0) > kMost || x.size(1) > kMost) NOT_MINE;
+  const at::ScalarType type = args[3] == Py_None ? x.scalar_type() : reinterpret_cast<THPDtype*>(args[3])->scalar_type;
+  if (type != at::kHalf && type != at::kFloat && type != at::kBFloat16) NOT_MINE;
+  at::Tensor y = rows_like(x, x.size(0), x.size(1), type);
+  if (lib.norm(ptr(x), x.stride(0), float_type(x), ptr(w), w.defined() ? float_type(w) : 1, (float)number(args[2]), (int)x.size(0), (int)x.size(1), ptr(y), float_type(y), current_stream(device)))
+    return failed();
+  return wrap(y);
+  END_HANDLE_TH_ERRORS
+}
+
+// grad_y, x, weight, eps, grad_residual
+PyObject* block_norm_backward(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
+  ARGS(5);
+  const at::Tensor &g = tensor(args[0], ok), &x = tensor(args[1], ok), &w = tensor(args[2], ok), &gr = tensor(args[4], ok);
+  if (!ok || !g.defined() || !x.defined() || !x.is_cuda()) NOT_MINE;
+  const int device = current_device();
+  if (!rows(x, device) || !rows(g, device, x.size(0), x.size(1)) || (w.defined() && !vector(w, device, x.size(1))) || x.size(0) > kMost || x.size(1) > kMost ||
+      (gr.defined() && (!rows(gr, device, x.size(0), x.size(1)) || gr.scalar_type() != x.scalar_type())))
+    NOT_MINE;
+  at::Tensor grad_x = rows_like(x, x.size(0), x.size(1), x.scalar_type()), grad_w, ws;
+  if (w.defined()) {
+    grad_w = at::empty({x.size(1)}, w.options().requires_grad(false));
+    ws = bytes(x, lib.backward_workspace((int)x.size(0), (int)x.size(1)));
+  }
+  if (lib.norm_backward(ptr(g), g.stride(0), float_type(g), ptr(x), x.stride(0), float_type(x), ptr(w), w.defined() ? float_type(w) : 1, ptr(gr), ld(gr), (float)number(args[3]), (int)x.size(0),
+                        (int)x.size(1), ptr(grad_x), ptr(grad_w), ptr(ws), current_stream(device)))
+    return failed();
+  return tuple(grad_x, grad_w);
+  END_HANDLE_TH_ERRORS
+}
+
+// What block_residual and its backward take alike: x, z, gate, gate_act, scale, norm_weight, next_weight
+struct ResidualInputs {
+  int device = 0;
+  const at::Tensor *x, *z, *gate, *scale, *w1, *w2;
+  int gate_kind = 0, sigmoid = 0, wtype = 1;
+  float factor = 1.0f;
+  bool read(PyObject* const* a) {
+    bool ok = true;
+    x = &tensor(a[0], ok);
+    z = &tensor(a[1], ok);
+    gate = &tensor(a[2], ok);
+    scale = a[4] == Py_None || PyFloat_Check(a[4]) ? &kNone : &tensor(a[4], ok);
+    w1 = &tensor(a[5], ok);
+    w2 = &tensor(a[6], ok);
+    if (!ok || !x->defined() || !z->defined() || !x->is_cuda()) return false;
+    device = current_device();
+    if (!rows(*x, device) || x->size(0) > kMost || x->size(1) > kMost || !rows(*z, device, x->size(0), x->size(1))) return false;
+    if (a[3] != Py_None) {
+      if (!PyUnicode_Check(a[3]) || PyUnicode_CompareWithASCIIString(a[3], "sigmoid") != 0) return false;
+      sigmoid = gate->defined();
+    }
+    if (PyFloat_Check(a[4])) factor = (float)PyFloat_AS_DOUBLE(a[4]);
+    const int64_t t = x->size(0), k = x->size(1);
+    if (gate->defined()) {
+      if (gate->dim() < 1 || gate->size(0) != t || !on(*gate, device) || float_type(*gate) < 0) return false;
+      if (gate->dim() == 1 || (gate->dim() == 2 && gate->size(1) == 1)) gate_kind = 1;
+      else if (rows(*gate, device, t, k) && gate->scalar_type() == z->scalar_type()) gate_kind = 2;
+      else return false;
+    }
+    bool typed = false;
+    for (const at::Tensor* v : {scale, w1, w2}) {
+      if (!v->defined()) continue;
+      if (!vector(*v, device, k) || (typed && float_type(*v) != wtype)) return false;
+      wtype = float_type(*v);
+      typed = true;
+    }
+    return true;
+  }
+};
+
+// x, z, gate, gate_act, scale, norm_weight, next_weight, eps
+PyObject* block_residual(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
+  ARGS(8);
+  ResidualInputs in;
+  if (!in.read(args) || wants_grad({in.x, in.z, in.gate, in.scale, in.w1, in.w2})) NOT_MINE;
+  const int device = in.device;
+  const at::Tensor &x = *in.x, &z = *in.z, &gate = *in.gate;
+  const int64_t t = x.size(0), k = x.size(1);
+  at::Tensor h = rows_like(x, t, k, x.scalar_type()), y;
+  if (in.w2->defined()) y = rows_like(z, t, k, z.scalar_type());
+  if (lib.residual(ptr(x), x.stride(0), float_type(x), ptr(z), z.stride(0), float_type(z), in.gate_kind, ptr(gate), ld(gate), gate.defined() ? float_type(gate) : 1, in.sigmoid, in.factor,
+                   ptr(*in.scale), ptr(*in.w1), ptr(*in.w2), in.wtype, (float)number(args[7]), (int)t, (int)k, ptr(h), ptr(y), current_stream(device)))
+    return failed();
+  return y.defined() ? tuple(h, y) : wrap(h);
+  END_HANDLE_TH_ERRORS
+}
+
+// grad_h, grad_y, x, z, gate, gate_act, scale, norm_weight, next_weight, eps
+PyObject* block_residual_backward(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
+  ARGS(10);
+  const at::Tensor &gh = tensor(args[0], ok), &gy = tensor(args[1], ok);
+  ResidualInputs in;
+  if (!ok || !in.read(args + 2) || (!gh.defined() && !gy.defined()) || (gy.defined() && !in.w2->defined())) NOT_MINE;
+  const int device = in.device;
+  const at::Tensor &x = *in.x, &z = *in.z, &gate = *in.gate;
+  const int64_t t = x.size(0), k = x.size(1);
+  if ((gh.defined() && (!rows(gh, device, t, k) || gh.scalar_type() != x.scalar_type())) || (gy.defined() && (!rows(gy, device, t, k) || gy.scalar_type() != z.scalar_type()))) NOT_MINE;
+  at::Tensor grad_x = rows_like(x, t, k, x.scalar_type()), grad_z = rows_like(z, t, k, z.scalar_type()), grad_gate, grad_scale, grad_w1, grad_w2, ws;
+  if (gate.defined()) grad_gate = at::empty(gate.sizes(), gate.options().requires_grad(false));
+  if (in.scale->defined()) grad_scale = at::empty({k}, in.scale->options().requires_grad(false));
+  if (in.w1->defined()) grad_w1 = at::empty({k}, in.w1->options().requires_grad(false));
+  if (in.w2->defined()) grad_w2 = at::empty({k}, in.w2->options().requires_grad(false));
+  if (grad_scale.defined() || grad_w1.defined() || grad_w2.defined()) ws = bytes(x, lib.backward_workspace((int)t, (int)k));
+  if (lib.residual_backward(ptr(gh), ld(gh), ptr(gy), ld(gy), ptr(x), x.stride(0), float_type(x), ptr(z), z.stride(0), float_type(z), in.gate_kind, ptr(gate), ld(gate),
+                            gate.defined() ? float_type(gate) : 1, in.sigmoid, in.factor, ptr(*in.scale), ptr(*in.w1), ptr(*in.w2), in.wtype, (float)number(args[9]), (int)t, (int)k, ptr(grad_x),
+                            ptr(grad_z), ptr(grad_gate), ptr(grad_scale), ptr(grad_w1), ptr(grad_w2), ptr(ws), current_stream(device)))
+    return failed();
+  return tuple(grad_x, grad_z, grad_gate, grad_scale, grad_w1, grad_w2);
+  END_HANDLE_TH_ERRORS
+}
+
+// bind(addresses of the library's entry points in the order of Library, torch's getter of the current device, of a device's current stream)
+PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
+  constexpr Py_ssize_t kPointers = sizeof(Library) / sizeof(void*);
+  if (n_args != kPointers + 2) {
+    PyErr_SetString(PyExc_TypeError, "bind: the library's entry points, a getter of the device and one of the stream");
+    return nullptr;
+  }
+  void* p[kPointers];
+  for (Py_ssize_t i = 0; i < kPointers; ++i) {
+    p[i] = PyLong_AsVoidPtr(args[i]);
+    if (PyErr_Occurred()) return nullptr;
+  }
+  Py_XDECREF(get_device);
+  Py_XDECREF(get_stream);
+  Py_INCREF(get_device = args[kPointers]);
+  Py_INCREF(get_stream = args[kPointers + 1]);
+  static_assert(sizeof p == sizeof lib, "one pointer each");
+  memcpy(&lib, p, sizeof lib);
+  Py_RETURN_NONE;
+}
+
+#define METHOD(name) {#name, (PyCFunction)(void*)name, METH_FASTCALL, nullptr}
+PyMethodDef methods[] = {METHOD(bind), METHOD(permute_tokens), METHOD(unpermute_tokens), METHOD(unpermute_tokens_backward), METHOD(route_topk_backward), METHOD(block_norm),
+                         METHOD(block_norm_backward), METHOD(block_residual), METHOD(block_residual_backward), {nullptr, nullptr, 0, nullptr}};
+PyModuleDef module = {PyModuleDef_HEAD_INIT, "_block_calls", nullptr, -1, methods};
+
+}  // namespace
+
+PyMODINIT_FUNC PyInit__block_calls() { return PyModule_Create(&module); }

@@ -477,6 +477,40 @@ def test_a_block_of_experts_trained_through():
         assert (a.double() - b).norm() <= 2 ** -24 * 2000 * b.norm(), name
 
 
+def test_calls_in_python_and_in_the_extension_are_the_same(monkeypatch):
+    """Every operator once with its host side in the extension and once in Python, with numbers of either kind for the residual scale."""
+    from mxmoe_amd import block, ops
+
+    class Nothing:
+        def __getattr__(self, name):
+            return lambda *a: None
+
+    taken = []
+
+    class Counted:
+        def __getattr__(self, name):
+            def call(*a):
+                got = getattr(native, name)(*a)
+                taken.append((name, got is not None))
+                return got
+
+            return call
+
+    ops.block_norm(_rnd(1, 8))
+    native = block._fast
+    s = _state(3)
+    monkeypatch.setattr(block, "_fast", Counted())
+    want = _all_operators(s)
+    scaled = [ops.block_residual(s["x"], s["x"], scale=c) for c in (2.0, 2, None)]
+    assert len({name for name, ok in taken if ok}) == 8 and [ok for name, ok in taken if name == "block_residual"] == [True, True, False, True]
+    monkeypatch.setattr(block, "_fast", Nothing())
+    for a, b in zip(_all_operators(s), want):
+        assert torch.equal(a, b) and a.dtype == b.dtype and a.shape == b.shape and a.stride() == b.stride()
+    for c, b in zip((2.0, 2, None), scaled):
+        assert torch.equal(ops.block_residual(s["x"], s["x"], scale=c), b)
+        assert torch.equal(ops.block_residual(s["x"].clone().requires_grad_(), s["x"], scale=c).detach(), b)
+
+
 # ---- streams, graphs, refusals ----
 
 def _all_operators(s):
