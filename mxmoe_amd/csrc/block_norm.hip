@@ -16,7 +16,8 @@ template <typename TX, typename TZ, bool HAS_Z, int NT, int VPT>
 __global__ void __launch_bounds__(NT) block_norm_kernel(const BlockNormArgs a) {
   __shared__ float sums[2][NT / 64];
   const int K = a.K, C = (K + 7) >> 3;
-  const long t = blockIdx.x;
+  const long t = folded_block();
+  if (t >= a.T) return;
   typename Piece<TX>::raw x_raw[VPT];
   typename Piece<TZ>::raw z_raw[HAS_Z ? VPT : 1], g_raw[HAS_Z ? VPT : 1];
 #pragma unroll
@@ -35,7 +36,7 @@ __global__ void __launch_bounds__(NT) block_norm_kernel(const BlockNormArgs a) {
   }
   f8 h[VPT];
 #pragma unroll
-  for (int v = 0; v < VPT; ++v) h[v] = Piece<TX>::widen(x_raw[v]);
+  for (int v = 0; v < VPT; ++v) h[v] = widen_piece<TX>(x_raw[v], threadIdx.x + v * NT, K);
   if constexpr (HAS_Z) {
     float row = a.factor;  // what the whole row is multiplied by: the residual scale, a token's gate, r_z
     if (a.gate_kind == kTokenGate) {
@@ -46,7 +47,7 @@ __global__ void __launch_bounds__(NT) block_norm_kernel(const BlockNormArgs a) {
       float sq[1] = {0.0f};
 #pragma unroll
       for (int v = 0; v < VPT; ++v) {
-        const f8 z = Piece<TZ>::widen(z_raw[v]);
+        const f8 z = widen_piece<TZ>(z_raw[v], threadIdx.x + v * NT, K);
         sq[0] = dot8(z, z, sq[0]);
       }
       group_sum<NT, 1>(sq, sums[0]);
@@ -56,11 +57,11 @@ __global__ void __launch_bounds__(NT) block_norm_kernel(const BlockNormArgs a) {
     for (int v = 0; v < VPT; ++v) {
       const int c = threadIdx.x + v * NT;
       if (c < C) {
-        f8 n = row * Piece<TZ>::widen(z_raw[v]);
+        f8 n = row * widen_piece<TZ>(z_raw[v], c, K);
         if (a.w1) n *= load_piece_of(a.wtype, a.w1, c, K);
         if (a.scale) n *= load_piece_of(a.wtype, a.scale, c, K);
         if (a.gate_kind == kElementGate) {
-          const f8 g = Piece<TZ>::widen(g_raw[v]);
+          const f8 g = widen_piece<TZ>(g_raw[v], c, K);
 #pragma unroll
           for (int e = 0; e < 8; ++e) n[e] *= a.sigmoid ? Sigmoid(g[e]).a : g[e];
         }
@@ -95,7 +96,7 @@ template <typename TX, typename TZ, bool HAS_Z>
 static void run_block_norm(const BlockNormArgs& a, hipStream_t s) {
   const int C = (a.K + 7) / 8;
   // threads a row: one wave up to 128 pieces (no barrier), then four waves, for very long rows sixteen
-#define RUN(NT, VPT) hipLaunchKernelGGL((block_norm_kernel<TX, TZ, HAS_Z, NT, VPT>), dim3(a.T), dim3(NT), 0, s, a)
+#define RUN(NT, VPT) hipLaunchKernelGGL((block_norm_kernel<TX, TZ, HAS_Z, NT, VPT>), folded_grid(a.T), dim3(NT), 0, s, a)
   if (C <= 128) RUN(64, 2);
   else if (C <= 256) RUN(256, 1);
   else if (C <= 512) RUN(256, 2);

@@ -46,14 +46,17 @@ __global__ void __launch_bounds__(1024) column_sum_kernel(const ColumnSumArgs a)
   }
 }
 
-static int run_backward(int xtype, int ztype, bool has_z, const BlockNormArgs& a, void* grad_w2, void* grad_w1, void* grad_scale, hipStream_t s) {
+static int run_backward(int xtype, int ztype, bool has_z, BlockNormArgs& a, void* grad_w2, void* grad_w1, void* grad_scale, hipStream_t s) {
+  a.grad_w2 = grad_w2;
+  a.grad_w1 = grad_w1;
+  a.grad_scale = grad_scale;
   const int grid = backward_groups(a.T, a.K);
   if (grid > 0) {
     if (xtype == kF16) run_block_backward<_Float16>(ztype, has_z, a, grid, s);
     else if (xtype == kF32) run_block_backward<float>(ztype, has_z, a, grid, s);
     else run_block_backward<__bf16>(ztype, has_z, a, grid, s);
   }
-  if (grad_w2 || grad_w1 || grad_scale) {  // (no tokens: the sums are zero, and are written)
+  if (grid != 1 && (grad_w2 || grad_w1 || grad_scale)) {  // (no tokens: the sums are zero, and are written)
     const int planes = has_z ? 2 : 1;
     const ColumnSumArgs c{a.partial, grid, planes, a.K, a.wtype, a.factor, a.scale, a.w1, grad_w2, grad_w1, grad_scale};
     hipLaunchKernelGGL(column_sum_kernel, dim3((a.K + 31) / 32, planes), dim3(1024), 0, s, c);
@@ -76,7 +79,8 @@ extern "C" {
 
 size_t mxmoe_block_backward_workspace_bytes(int num_tokens, int K) {
   if (num_tokens <= 0 || K < 1 || K > kMaxNormRow) return 0;
-  return (size_t)backward_groups(num_tokens, K) * 2 * (size_t)K * sizeof(float);
+  const int groups = backward_groups(num_tokens, K);
+  return groups > 1 ? (size_t)groups * 2 * (size_t)K * sizeof(float) : 0;
 }
 
 int mxmoe_block_norm_backward(const void* grad_y, int64_t ld_grad_y, int y_dtype, const void* x, int64_t ldx, int x_dtype, const void* weight, int weight_dtype, const void* grad_residual,
@@ -97,7 +101,7 @@ int mxmoe_block_norm_backward(const void* grad_y, int64_t ld_grad_y, int y_dtype
   a.grad_x = grad_x;
   a.partial = reinterpret_cast<float*>(workspace);
   if (const int rc = check_block_norm(a, x_dtype, y_dtype)) return rc;
-  if ((weight && !grad_weight) || (num_tokens && (!grad_y || !x || !grad_x || (weight && !workspace)))) return null_pointer();
+  if ((weight && !grad_weight) || (num_tokens && (!grad_y || !x || !grad_x || (weight && !workspace && mxmoe_block_backward_workspace_bytes(num_tokens, K))))) return null_pointer();
   return run_backward(x_dtype, y_dtype, false, a, weight ? grad_weight : nullptr, nullptr, nullptr, (hipStream_t)stream);
 }
 
@@ -137,7 +141,7 @@ int mxmoe_block_residual_backward(const void* grad_h, int64_t ld_grad_h, const v
     return 3;
   }
   if ((scale && !grad_scale) || (norm_weight && !grad_norm_weight) || (next_weight && !grad_next_weight)) return null_pointer();
-  if (num_tokens && (!x || !z || !grad_x || !grad_z || (gate_kind && !grad_gate) || ((scale || norm_weight || next_weight) && !workspace))) return null_pointer();
+  if (num_tokens && (!x || !z || !grad_x || !grad_z || (gate_kind && !grad_gate) || ((scale || norm_weight || next_weight) && !workspace && mxmoe_block_backward_workspace_bytes(num_tokens, K)))) return null_pointer();
   if (num_tokens && !grad_h && !grad_y) {
     last_error() = "neither the gradient of h nor that of y is given";
     return 5;

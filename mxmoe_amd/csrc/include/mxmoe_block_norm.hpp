@@ -37,6 +37,9 @@ struct BlockNormArgs {
   void* grad_x;
   void* grad_z;
   void* grad_gate;
+  void* grad_w2;          // written by the kernel itself where one workgroup has all tokens
+  void* grad_w1;
+  void* grad_scale;
   float* partial;         // [grid][2][K]: sums over the workgroup's tokens of grad_y h r_h, and of grad_h' a z r_z
 };
 
@@ -63,12 +66,17 @@ __device__ __forceinline__ float rms_factor(float sum, float inv_k, float eps) {
   return __builtin_amdgcn_rsqf(v);
 }
 
-// Threads a row: one piece a thread up to rows of 8192, so that a workgroup's columns fit its registers.
-inline int backward_threads(int K) { return K <= 512 ? 64 : K <= 1024 ? 128 : K <= 2048 ? 256 : K <= 4096 ? 512 : 1024; }
-// Workgroups: as many as the card holds at once, each with the same number of tokens or one less
+// Tokens that one workgroup takes alone, so that the launch that adds up the workgroups' sums is left out (4 tokens of 2048, all options: 10.9 us against 8.0, and 3 us
+// less of the host's time, which bounds such a call; 8 tokens: 18 against 8.0)
+constexpr int kAloneTokens = 4;
+// Workgroups of the backward kernel: as many as the card holds at once (for rows past 2048 one a CU; a second one, with fewer registers, took 145 us where one takes 119:
+// 8192 tokens of 4096), each with the same number of tokens or one less, and from 512 tokens on with two at least, which halves the sums to be added up
+// (512 tokens of 2048: 14.0 -> 12.8 us)
 inline int backward_groups(int T, int K) {
-  const int most = std::max(256, 131072 / backward_threads(K));
-  return T < most ? T : (T + (T + most - 1) / most - 1) / ((T + most - 1) / most);
+  if (T <= kAloneTokens) return T > 0;
+  const int most = K <= 2048 ? 512 : 256, teams = K <= 512 ? 4 : 1;  // (rows of up to 512 go a wave each)
+  const int per = (std::max((T + most - 1) / most, T >= 512 ? 2 : 1) + teams - 1) / teams * teams;
+  return (T + per - 1) / per;
 }
 
 // one definition per type of x (block_norm_grad_*.hip)

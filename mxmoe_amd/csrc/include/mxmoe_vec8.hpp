@@ -11,7 +11,7 @@
 namespace mxmoe {
 
 // Eight values in registers of their own: a vector type of eight would hold eight neighbouring registers wherever it lives across a branch (175 registers instead of
-// REGS in the largest kernel).
+// 146 in the backward kernel of the norms).
 struct f8 {
   float v[8];
   f8() = default;
@@ -94,20 +94,54 @@ struct Piece<float> {
 // partial sums that the next launch reads, are cached.
 enum Caching { kStreamed, kCached };
 
-// elements 8 c .. 8 c + 7 of a row of K elements, zeros past its end; WHOLE: K is a multiple of eight (a kernel short of registers has both forms)
+// v moved down by n of its elements (0 < n < 8), zeros behind
+template <typename RAW>
+__device__ __forceinline__ RAW moved_down(RAW v, int n) {
+#pragma unroll
+  for (int step = 4; step > 0; step >>= 1) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = n & step ? (i + step < 8 ? v[i + step] : 0) : v[i];
+  }
+  return v;
+}
+// the same of 16-bit elements, as two 64-bit words
+template <typename RAW>
+__device__ __forceinline__ RAW moved_down_16(RAW v, int n) {
+  uint64_t w[2];
+  __builtin_memcpy(w, &v, 16);
+  const int bits = 16 * (n & 3);
+  const uint64_t lo = n & 4 ? w[1] : w[0], hi = n & 4 ? 0 : w[1];
+  w[0] = (lo >> bits) | (bits ? hi << (64 - bits) : 0);
+  w[1] = hi >> bits;
+  __builtin_memcpy(&v, w, 16);
+  return v;
+}
+
+// Elements 8 c .. 8 c + 7 of a row of K elements; WHOLE: K is a multiple of eight (a kernel short of registers has both forms).  Where the row ends inside the piece, its last
+// eight elements are loaded instead, one trip to memory as for any other piece, and widen_piece moves them into place with zeros behind: in two steps, because the
+// second waits for the data, and a row's kernel has several loads to issue first.
 template <typename T, bool WHOLE = false, int CACHING = kStreamed>
 __device__ __forceinline__ typename Piece<T>::raw load_piece(const T* row, int c, int K) {
   typename Piece<T>::raw v{};
-  if (WHOLE || 8 * c + 8 <= K) {
-    const auto* p = reinterpret_cast<const typename Piece<T>::mem*>(row + 8 * c);
+  const int first = WHOLE ? 8 * c : min(8 * c, K - 8);
+  if (WHOLE || first >= 0) {
+    const auto* p = reinterpret_cast<const typename Piece<T>::mem*>(row + first);
     if constexpr (CACHING == kStreamed) v = __builtin_nontemporal_load(p);
     else v = *p;
-  } else {
+  } else {  // a row of less than eight elements
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      if (8 * c + i < K) v[i] = row[8 * c + i];
+      if (i < K) v[i] = row[i];
   }
   return v;
+}
+template <typename T, bool WHOLE = false>
+__device__ __forceinline__ f8 widen_piece(typename Piece<T>::raw v, int c, int K) {
+  if (!WHOLE && 8 * c + 8 > K && K >= 8) {
+    if constexpr (sizeof(T) == 2) v = moved_down_16(v, 8 * c + 8 - K);
+    else v = moved_down(v, 8 * c + 8 - K);
+  }
+  return Piece<T>::widen(v);
 }
 template <typename T, bool WHOLE = false, int CACHING = kStreamed>
 __device__ __forceinline__ void store_piece(T* row, int c, int K, typename Piece<T>::raw v) {
@@ -115,29 +149,51 @@ __device__ __forceinline__ void store_piece(T* row, int c, int K, typename Piece
     auto* p = reinterpret_cast<typename Piece<T>::mem*>(row + 8 * c);
     if constexpr (CACHING == kStreamed) __builtin_nontemporal_store(v, p);
     else *p = v;
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (8 * c + i < K) row[8 * c + i] = v[i];
+  } else {  // the row's last one to seven elements: four, two and one of them, as their number has it
+    typedef T quad __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+    typedef T pair __attribute__((ext_vector_type(2), aligned(sizeof(T))));
+    T* p = row + 8 * c;
+    const int n = K - 8 * c;
+    if (n & 4) {
+      *reinterpret_cast<quad*>(p) = quad{v[0], v[1], v[2], v[3]};
+      v = typename Piece<T>::raw{v[4], v[5], v[6]};
+      p += 4;
+    }
+    if (n & 2) {
+      *reinterpret_cast<pair*>(p) = pair{v[0], v[1]};
+      v[0] = v[2];
+      p += 2;
+    }
+    if (n & 1) *p = v[0];
   }
 }
 // the same of a vector whose type is known at run time only (norm weights: read once per workgroup, or from a cache)
 template <bool WHOLE = false>
 __device__ __forceinline__ f8 load_piece_of(int type, const void* row, int c, int K) {
-  if (type == kF32) return Piece<float>::widen(load_piece<float, WHOLE, kCached>(reinterpret_cast<const float*>(row), c, K));
-  if (type == kF16) return Piece<_Float16>::widen(load_piece<_Float16, WHOLE, kCached>(reinterpret_cast<const _Float16*>(row), c, K));
-  return Piece<__bf16>::widen(load_piece<__bf16, WHOLE, kCached>(reinterpret_cast<const __bf16*>(row), c, K));
+  if (type == kF32) return widen_piece<float, WHOLE>(load_piece<float, WHOLE, kCached>(reinterpret_cast<const float*>(row), c, K), c, K);
+  if (type == kF16) return widen_piece<_Float16, WHOLE>(load_piece<_Float16, WHOLE, kCached>(reinterpret_cast<const _Float16*>(row), c, K), c, K);
+  return widen_piece<__bf16, WHOLE>(load_piece<__bf16, WHOLE, kCached>(reinterpret_cast<const __bf16*>(row), c, K), c, K);
 }
 __device__ __forceinline__ float load_of(int type, const void* p, long i) {
   if (type == kF32) return reinterpret_cast<const float*>(p)[i];
   if (type == kF16) return (float)reinterpret_cast<const _Float16*>(p)[i];
   return (float)reinterpret_cast<const __bf16*>(p)[i];
 }
+template <bool WHOLE = false>
+__device__ __forceinline__ void store_piece_of(int type, void* row, int c, int K, const f8& v) {
+  if (type == kF32) store_piece<float, WHOLE, kCached>(reinterpret_cast<float*>(row), c, K, Piece<float>::narrow(v));
+  else if (type == kF16) store_piece<_Float16, WHOLE, kCached>(reinterpret_cast<_Float16*>(row), c, K, Piece<_Float16>::narrow(v));
+  else store_piece<__bf16, WHOLE, kCached>(reinterpret_cast<__bf16*>(row), c, K, Piece<__bf16>::narrow(v));
+}
 __device__ __forceinline__ void store_of(int type, void* p, long i, float v) {
   if (type == kF32) reinterpret_cast<float*>(p)[i] = v;
   else if (type == kF16) reinterpret_cast<_Float16*>(p)[i] = (_Float16)v;
   else reinterpret_cast<__bf16*>(p)[i] = (__bf16)v;
 }
+
+// Grids of a workgroup per token or so: a dimension holds less than 2^32 threads, which 2^26 short rows reach, so they are folded into rows of 2^20 workgroups.
+inline dim3 folded_grid(long workgroups) { return workgroups <= (1 << 20) ? dim3((unsigned)workgroups) : dim3(1 << 20, (unsigned)((workgroups + (1 << 20) - 1) >> 20)); }
+__device__ __forceinline__ long folded_block() { return (long)blockIdx.y * gridDim.x + blockIdx.x; }  // (past the last one in the last row)
 
 // Sum over the wave, in every lane: lanes of a row of 16 by shifts, rows by the broadcast of their last lanes; the vector ALU alone (a shuffle is
 // a round trip through LDS).  All 64 lanes must be active.

@@ -233,7 +233,8 @@ __global__ void __launch_bounds__(256) permute_kernel(const PermuteArgs a) {
 
 // ---- unpermute, and permute's backward ----
 //
-// `tpt` threads a token (whole waves, so that a token's rows and weights are scalars), 16 bytes of every row at a time, up to eight slots' loads in flight.
+// `tpt` threads a token, 16 bytes of every row at a time, up to eight slots' loads in flight.  Whole waves (tpt of 64 and more) have a token's rows and weights as scalars;
+// short rows go several tokens to a wave.
 // Products and sums are rounded one by one in slot order, as combine_kernel's: the same bits for fp16.
 struct GatherArgs {
   const void* rows;
@@ -246,11 +247,16 @@ struct GatherArgs {
   int T, topk, K, tpt;
   void* out;
 };
-template <typename T>
+template <typename T, bool WAVES>
 __global__ void __launch_bounds__(256) unpermute_kernel(const GatherArgs a) {
   constexpr int kSlots = 8;
-  const int team = __builtin_amdgcn_readfirstlane((int)threadIdx.x / a.tpt);
-  const int t = blockIdx.x * (256 / a.tpt) + team;
+  auto of_token = [](const auto* p) {
+    if constexpr (WAVES) return const_load(p);
+    else return *p;
+  };
+  int team = (int)threadIdx.x / a.tpt;
+  if constexpr (WAVES) team = __builtin_amdgcn_readfirstlane(team);
+  const long t = folded_block() * (256 / a.tpt) + team;
   if (t >= a.T) return;  // (no barrier below)
   const int C = (a.K + 7) >> 3;
   for (int c = threadIdx.x % a.tpt; c < C; c += a.tpt) {
@@ -261,19 +267,19 @@ __global__ void __launch_bounds__(256) unpermute_kernel(const GatherArgs a) {
       int r[kSlots];
       typename Piece<T>::raw v[kSlots];
 #pragma unroll
-      for (int i = 0; i < kSlots; ++i) r[i] = s0 + i < a.topk ? const_load(a.row_of_slot + (long)t * a.topk + s0 + i) : -1;
+      for (int i = 0; i < kSlots; ++i) r[i] = s0 + i < a.topk ? of_token(a.row_of_slot + t * a.topk + s0 + i) : -1;
 #pragma unroll
       for (int i = 0; i < kSlots; ++i)
         if (r[i] >= 0 && r[i] < a.num_rows) v[i] = load_piece(reinterpret_cast<const T*>(a.rows) + r[i] * a.ld, c, a.K);
 #pragma unroll
       for (int i = 0; i < kSlots; ++i)
         if (r[i] >= 0 && r[i] < a.num_rows) {
-          const f8 x = Piece<T>::widen(v[i]);
-          acc = acc + (a.weights ? const_load(a.weights + (long)t * a.topk + s0 + i) * x : x);
+          const f8 x = widen_piece<T>(v[i], c, a.K);
+          acc = acc + (a.weights ? of_token(a.weights + t * a.topk + s0 + i) * x : x);
         }
     }
-    if (a.shared) acc = acc + Piece<T>::widen(sh);
-    store_piece(reinterpret_cast<T*>(a.out) + (long)t * a.K, c, a.K, Piece<T>::narrow(acc));
+    if (a.shared) acc = acc + widen_piece<T>(sh, c, a.K);
+    store_piece(reinterpret_cast<T*>(a.out) + t * a.K, c, a.K, Piece<T>::narrow(acc));
   }
 }
 
@@ -289,21 +295,23 @@ struct UngatherArgs {
   int num_rows;
   const int32_t* row_of_slot;
   const float* weights;
-  int topk, K, keep_tail;
+  int T, topk, K, keep_tail;
   void* grad_rows;
   float* grad_weights;    // or null
 };
 template <typename T, int NT, int S>
 __global__ void __launch_bounds__(NT) unpermute_backward_kernel(const UngatherArgs a) {
   __shared__ float sums[2][S * (NT / 64)];
-  const int t = blockIdx.x, C = (a.K + 7) >> 3;
+  const long t = folded_block();
+  const int C = (a.K + 7) >> 3;
+  if (t >= a.T) return;
   const T* g_row = reinterpret_cast<const T*>(a.grad_out) + t * a.ld_grad;
   for (int s0 = 0, turn = 0; s0 < a.topk; s0 += S, turn ^= 1) {
     int r[S];
     float w[S], dot[S];
 #pragma unroll
     for (int i = 0; i < S; ++i) {
-      const long at = (long)t * a.topk + s0 + i;
+      const long at = t * a.topk + s0 + i;
       r[i] = s0 + i < a.topk ? const_load(a.row_of_slot + at) : -1;
       w[i] = s0 + i < a.topk && a.weights ? const_load(a.weights + at) : 1.0f;
       dot[i] = 0.0f;
@@ -316,12 +324,12 @@ __global__ void __launch_bounds__(NT) unpermute_backward_kernel(const UngatherAr
         for (int i = 0; i < S; ++i)
           if (r[i] >= 0 && r[i] < a.num_rows) v[i] = load_piece(reinterpret_cast<const T*>(a.rows) + r[i] * a.ld, c, a.K);
       }
-      const f8 g = Piece<T>::widen(g_raw);
+      const f8 g = widen_piece<T>(g_raw, c, a.K);
 #pragma unroll
       for (int i = 0; i < S; ++i) {
         if (r[i] >= 0 && r[i] < a.num_rows) {
           if (a.grad_weights) {
-            const f8 x = Piece<T>::widen(v[i]);
+            const f8 x = widen_piece<T>(v[i], c, a.K);
 #pragma unroll
             for (int e = 0; e < 8; ++e) dot[i] = __builtin_fmaf(g[e], x[e], dot[i]);
           }
@@ -335,7 +343,7 @@ __global__ void __launch_bounds__(NT) unpermute_backward_kernel(const UngatherAr
     group_sum<NT, S>(dot, sums[turn]);
 #pragma unroll
     for (int i = 0; i < S; ++i)
-      if ((int)threadIdx.x == i && s0 + i < a.topk) a.grad_weights[(long)t * a.topk + s0 + i] = dot[i];
+      if ((int)threadIdx.x == i && s0 + i < a.topk) a.grad_weights[t * a.topk + s0 + i] = dot[i];
   }
 }
 
@@ -371,12 +379,13 @@ __device__ __forceinline__ float team_sum(float v) {
 }
 template <int G, int R>
 __global__ void __launch_bounds__(256) route_backward_kernel(const RouteGradArgs a) {
-  const int g = threadIdx.x & (G - 1), t = blockIdx.x * (256 / G) + (int)threadIdx.x / G;
+  const int g = threadIdx.x & (G - 1);
+  const long t = folded_block() * (256 / G) + (int)threadIdx.x / G;
   const bool live = t < a.T;  // (lanes without a token go along: the sums run over whole teams)
-  const long base = (long)t * a.E;
+  const long base = t * a.E;
   const bool slot = live && g < a.topk;
-  const int id = slot ? a.ids[(long)t * a.topk + g] : -1;
-  const float dw = slot ? a.grad_weights[(long)t * a.topk + g] : 0.0f;
+  const int id = slot ? a.ids[t * a.topk + g] : -1;
+  const float dw = slot ? a.grad_weights[t * a.topk + g] : 0.0f;
   float x[R], d[R], n[R];
 #pragma unroll
   for (int i = 0; i < R; ++i) {
@@ -451,18 +460,20 @@ static int run_permute(PermuteArgs& a, int32_t* table, hipStream_t s) {
 
 template <typename T>
 static void run_unpermute(const GatherArgs& a, hipStream_t s) {
-  hipLaunchKernelGGL(unpermute_kernel<T>, dim3((a.T + 256 / a.tpt - 1) / (256 / a.tpt)), dim3(256), 0, s, a);
+  const dim3 grid = folded_grid((a.T + 256 / a.tpt - 1) / (256 / a.tpt));
+  if (a.tpt < 64) hipLaunchKernelGGL((unpermute_kernel<T, false>), grid, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((unpermute_kernel<T, true>), grid, dim3(256), 0, s, a);
 }
 template <typename T, int NT>
-static void run_unpermute_backward_as(const UngatherArgs& a, int num_tokens, hipStream_t s) {
-  if (a.topk <= 2) hipLaunchKernelGGL((unpermute_backward_kernel<T, NT, 2>), dim3(num_tokens), dim3(NT), 0, s, a);
-  else if (a.topk <= 4) hipLaunchKernelGGL((unpermute_backward_kernel<T, NT, 4>), dim3(num_tokens), dim3(NT), 0, s, a);
-  else hipLaunchKernelGGL((unpermute_backward_kernel<T, NT, 8>), dim3(num_tokens), dim3(NT), 0, s, a);
+static void run_unpermute_backward_as(const UngatherArgs& a, hipStream_t s) {
+  if (a.topk <= 2) hipLaunchKernelGGL((unpermute_backward_kernel<T, NT, 2>), folded_grid(a.T), dim3(NT), 0, s, a);
+  else if (a.topk <= 4) hipLaunchKernelGGL((unpermute_backward_kernel<T, NT, 4>), folded_grid(a.T), dim3(NT), 0, s, a);
+  else hipLaunchKernelGGL((unpermute_backward_kernel<T, NT, 8>), folded_grid(a.T), dim3(NT), 0, s, a);
 }
 template <typename T>
-static void run_unpermute_backward(const UngatherArgs& a, int num_tokens, hipStream_t s) {
-  if (a.K <= 1024) run_unpermute_backward_as<T, 64>(a, num_tokens, s);
-  else run_unpermute_backward_as<T, 256>(a, num_tokens, s);
+static void run_unpermute_backward(const UngatherArgs& a, hipStream_t s) {
+  if (a.K <= 1024) run_unpermute_backward_as<T, 64>(a, s);
+  else run_unpermute_backward_as<T, 256>(a, s);
 }
 
 static const char* kTokenSizes = "tokens sorted by expert: tokens >= 0, 1 <= topk <= 64, 1 <= experts <= 4096, K >= 1 and at most 2^30 (token, slot) pairs";
@@ -520,7 +531,7 @@ int mxmoe_unpermute_tokens(const void* rows, int64_t ld, int num_rows, const int
   if ((num_rows && !rows) || !row_of_slot || !out) return refuse(5, "null pointer");
   GatherArgs a{rows, (long)ld, num_rows, row_of_slot, topk_weights, shared, (long)ld_shared, num_tokens, topk, K, 0, out};
   const int C = (K + 7) / 8;
-  a.tpt = C <= 64 ? 64 : (C <= 128 ? 128 : 256);
+  a.tpt = C <= 8 ? 8 : C <= 16 ? 16 : C <= 32 ? 32 : C <= 64 ? 64 : C <= 128 ? 128 : 256;
   hipStream_t s = (hipStream_t)stream;
   if (dtype == kF16) run_unpermute<_Float16>(a, s);
   else if (dtype == kF32) run_unpermute<float>(a, s);
@@ -534,11 +545,11 @@ int mxmoe_unpermute_tokens_backward(const void* grad_out, int64_t ld_grad, const
   if (dtype < 0 || dtype > 2 || ld < 0 || ld_grad < 0) return refuse(3, "rows as fp16 (0), fp32 (1) or bf16 (2), row strides >= 0");
   if (num_tokens == 0) return 0;
   if (!grad_out || !row_of_slot || (num_rows && !grad_rows) || (grad_weights && num_rows && !rows)) return refuse(5, "null pointer");
-  const UngatherArgs a{grad_out, (long)ld_grad, rows, (long)ld, num_rows, row_of_slot, topk_weights, topk, K, keep_tail != 0, grad_rows, grad_weights};
+  const UngatherArgs a{grad_out, (long)ld_grad, rows, (long)ld, num_rows, row_of_slot, topk_weights, num_tokens, topk, K, keep_tail != 0, grad_rows, grad_weights};
   hipStream_t s = (hipStream_t)stream;
-  if (dtype == kF16) run_unpermute_backward<_Float16>(a, num_tokens, s);
-  else if (dtype == kF32) run_unpermute_backward<float>(a, num_tokens, s);
-  else run_unpermute_backward<__bf16>(a, num_tokens, s);
+  if (dtype == kF16) run_unpermute_backward<_Float16>(a, s);
+  else if (dtype == kF32) run_unpermute_backward<float>(a, s);
+  else run_unpermute_backward<__bf16>(a, s);
   return launched();
 }
 
@@ -551,7 +562,7 @@ int mxmoe_route_topk_backward(const float* grad_weights, const void* router_logi
   const RouteGradArgs a{grad_weights, router_logits, logits_dtype, topk_ids, num_tokens, num_experts, topk, renormalise != 0, grad_logits};
   hipStream_t s = (hipStream_t)stream;
   const int need = std::max(num_experts, topk);
-#define RUN(G, R) hipLaunchKernelGGL((route_backward_kernel<G, R>), dim3((unsigned)(((long)num_tokens * G + 255) / 256)), dim3(256), 0, s, a)
+#define RUN(G, R) hipLaunchKernelGGL((route_backward_kernel<G, R>), folded_grid(((long)num_tokens * G + 255) / 256), dim3(256), 0, s, a)
   if (need <= 8) RUN(8, 1);
   else if (need <= 16) RUN(16, 1);
   else if (need <= 32) RUN(32, 1);

@@ -168,7 +168,7 @@ def test_block_norms_refuse(lib):
     for bad in (dict(gy=None), dict(x=None), dict(gx=None), dict(gw=None), dict(ws=None)):
         assert nbwd(**bad) == 5, bad
     assert norm(t=0, x=None, y=None) == 0 and res(t=0, x=None, z=None, h=None) == 0
-    assert lib.mxmoe_block_backward_workspace_bytes(0, 64) == 0 and lib.mxmoe_block_backward_workspace_bytes(7, 64) == 7 * 2 * 64 * 4
+    assert lib.mxmoe_block_backward_workspace_bytes(0, 64) == 0 and lib.mxmoe_block_backward_workspace_bytes(7, 64) == 2 * 2 * 64 * 4
     assert lib.mxmoe_block_backward_workspace_bytes(3, 32769) == 0
 
 

@@ -192,6 +192,66 @@ def test_permutation_past_32_bit_offsets():
     assert torch.equal(h[-1], grad[-1] + 1) and torch.equal(y[-1], ops.block_norm(h[-1:])[0])
 
 
+def test_more_rows_than_a_grid_holds_threads():
+    """2^26 rows and some: a wave each would be 2^32 threads."""
+    from mxmoe_amd import ops
+
+    t = (1 << 26) + 77
+    x = torch.arange(t, device=DEV, dtype=torch.int32).bitwise_and(255).to(BF16)[:, None].expand(t, 8)
+    y = ops.block_norm(x, None, 1.0)
+    one = ops.block_norm(x[:256].contiguous(), None, 1.0)
+    assert torch.equal(y[-333:], one.repeat(3, 1)[(t - 333) % 256:][:333]) and torch.equal(y[::1001], one[(torch.arange(0, t, 1001, device=DEV)) % 256])
+    del y
+    m = torch.arange(t, device=DEV, dtype=torch.int32).bitwise_and(255)[:, None]
+    g = ops.unpermute_tokens_backward(x, x[:256].contiguous(), m, torch.ones(t, 1, device=DEV))[1]   # a wave a token
+    assert torch.equal(g[:, 0], 8 * m[:, 0].float() ** 2)
+    del g
+    ids = torch.ones(t, 1, device=DEV, dtype=torch.int32)
+    logits = torch.tensor([0.0, 1.0] + [-1.0] * 62, dtype=BF16, device=DEV).expand(t, 64).contiguous()
+    d = ops.route_topk_backward(torch.ones(t, 1, device=DEV), logits, ids)
+    assert torch.equal(d, d[:1].expand(t, 64)) and torch.equal(d[:1], ops.route_topk_backward(torch.ones(1, 1, device=DEV), logits[:1], ids[:1]))
+
+
+@pytest.mark.parametrize("width", [1, 5, 8, 12, 130, 515, 2055, 4100, 8200])
+@pytest.mark.parametrize("dtype", [F16, F32])
+def test_nothing_is_written_past_the_rows(width, dtype):
+    from mxmoe_amd import ops
+
+    t = 5
+
+    def guarded(rows, k, dt=dtype):
+        buf = torch.full((rows * k + 64,), 7.0, dtype=dt, device=DEV)
+        return buf, buf[32:32 + rows * k].view(rows, k)
+
+    def untouched(*bufs):
+        return all((b[:32] == 7).all() and (b[-32:] == 7).all() for b in bufs)
+
+    x, ids, w = _rnd(t, width, dtype=dtype, seed=1), _ids(t, 2, 3, 1), _rnd(t, 2, seed=2)
+    bufs, outs = zip(guarded(t * 2, width), guarded(t, width), guarded(t * 2, width), guarded(t, width), guarded(t, width))
+    rows, m, _ = ops.permute_tokens(x, ids, 3, out=outs[0])
+    ops.unpermute_tokens(rows, m, w, x, out=outs[1])
+    ops.unpermute_tokens_backward(x, rows, m, w, out=outs[2])
+    ops.block_norm(x, out=outs[3])
+    ops.block_residual(x, x, next_weight=x[0], out=outs[4])
+    assert untouched(*bufs)
+    # gradients, whose buffers the operators take themselves: the entry points with guarded ones
+    lib, s = _lib(), torch.cuda.current_stream().cuda_stream
+    code, f = {F16: 0, F32: 1}[dtype], torch.ones(width, dtype=dtype, device=DEV)
+    bufs, outs = zip(*(guarded(t, width) for _ in range(3)), *(guarded(1, width) for _ in range(3)), guarded(1, lib.mxmoe_block_backward_workspace_bytes(t, width) // 4, F32))
+    p = [o.data_ptr() for o in outs]
+    for tokens in (t, 3):
+        rc = lib.mxmoe_block_residual_backward(x.data_ptr(), width, x.data_ptr(), width, x.data_ptr(), width, code, x.data_ptr(), width, code, 2, x.data_ptr(), width, code, 1, 1.0,
+                                               f.data_ptr(), f.data_ptr(), f.data_ptr(), code, 1e-6, tokens, width, *p, s)
+        torch.cuda.synchronize()
+        assert rc == 0 and untouched(*bufs)
+
+
+def _lib():
+    from mxmoe_amd import _lib as L
+
+    return L.load()
+
+
 # ---- routing ----
 
 @pytest.mark.parametrize("t,e,k", [(1, 1, 1), (201, 8, 2), (33, 3, 3), (65, 60, 4), (130, 64, 6), (9, 65, 8), (21, 256, 8), (3, 4096, 64), (5, 100, 64)])
