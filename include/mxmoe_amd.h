@@ -317,7 +317,7 @@ int mxmoe_upload(void* dst, const void* host_src, size_t bytes, void* stream);
  *     gradient of mxmoe_permute_tokens is this call on the rows' gradients); shared NULL: none.
  * mxmoe_unpermute_tokens_backward   grad_rows[row(t, s)] = topk_weights[t, s] * grad_out[t], and zeros (keep_tail != 0: nothing) in the row that a
  *     dropped slot's entry -2 - row names (an entry -1 names none); grad_weights[t, s] = <grad_out[t], rows[row(t, s)]> in fp32, 0 for a dropped slot.
- *     topk_weights NULL: all 1; grad_weights NULL: not wanted, and rows
+ *     The map names every row at most once; a row that no entry names is not written.  topk_weights NULL: all 1; grad_weights NULL: not wanted, and rows
  *     is not read.  grad_shared is grad_out. */
 size_t mxmoe_permute_tokens_workspace_bytes(int num_tokens, int topk, int num_experts);
 int mxmoe_permute_tokens(const void* hidden, int64_t ld, int dtype, const void* topk_ids, int ids_bytes, int num_tokens, int topk, int num_experts, int K, void* rows, int keep_tail,

@@ -1,6 +1,6 @@
 // Backward kernel of the norms around a block (forward and notation: mxmoe_block_norm.hpp), instantiated per type of the residual stream.
 //
-//   c1  = r_h^3 / K  sum grad_y w2 h                     D  = grad_h + r_h grad_y w2 - c1 h            (grad_x = D)
+//   hh  = h r_h,  c1 = r_h^2 / K  sum grad_y w2 h        D  = grad_h + r_h grad_y w2 - c1 hh           (grad_x = D; r_h^3 would leave fp32's range before D does)
 //   c2  = sum D s n (gate per element inside, per token outside the sum)
 //   grad_z    = r_z (D s a w1 - z r_z  c2 a_token / K)   or D s a without a norm behind the block
 //   grad_gate = c2 act' per token,  D s n act' per element
@@ -160,10 +160,10 @@ __global__ void __launch_bounds__(NT * TEAMS) block_norm_backward_kernel(const B
     }
     if (a.grad_y) {
       r_h = rms_factor(s[0], inv_k, a.eps);
-      c1 = r_h * r_h * r_h * s[1] * inv_k;
+      c1 = r_h * (r_h * s[1] * inv_k);
     }
     if constexpr (HAS_Z) {
-      c2 = s[2] + r_h * s[3] - c1 * s[4];
+      c2 = s[2] + r_h * s[3] - c1 * (r_h * s[4]);
       if (a.w1) c3 = a_token * c2 * inv_k;
       if (a.gate_kind == kTokenGate && tid == 0) store_of(a.gate_type, a.grad_gate, t, c2 * slope_token);
     }
@@ -173,8 +173,9 @@ __global__ void __launch_bounds__(NT * TEAMS) block_norm_backward_kernel(const B
       const bool mine = 8 * c < K;
       f8 D = gh[v];
       if (a.grad_y) {
-        D = fma8(r_h, dyw[v], fma8(-c1, h[v], D));
-        P[v] = fma8(gy[v], r_h * h[v], P[v]);
+        const f8 hh = r_h * h[v];
+        D = fma8(r_h, dyw[v], fma8(-c1, hh, D));
+        P[v] = fma8(gy[v], hh, P[v]);
       }
       if (mine) store_piece<TX, WHOLE>(reinterpret_cast<TX*>(a.grad_x) + t * K, c, K, Piece<TX>::narrow(D));
       if constexpr (HAS_Z) {

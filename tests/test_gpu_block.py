@@ -149,6 +149,9 @@ def test_unpermute_tokens_maps_of_the_other_permutation_and_bad_ones():
     routed = int((m >= 0).sum())
     a, b = ops.unpermute_tokens_backward(g, y, other, w), ops.unpermute_tokens_backward(g, y, m, w)
     assert torch.equal(a[0][:routed], b[0][:routed]) and torch.equal(a[1], b[1])
+    more = torch.cat([y, y[:5]])                                                               # (rows that no slot can name)
+    c = ops.unpermute_tokens_backward(g, more, m, w)
+    assert torch.equal(c[0][:60], b[0]) and not c[0][60:].any() and torch.equal(c[1], b[1])
     # entries past the rows that there are name nothing, in either sign
     bad = m.clone()
     bad[0] = torch.tensor([60, 2 ** 31 - 1, -2 ** 31], dtype=torch.int32)
@@ -431,6 +434,11 @@ def test_norms_of_zeros_infinities_and_large_values():
     y = ops.block_norm(x, None, 1e-6)
     assert not y[0].any() and (y[1] == 1).all() and torch.isnan(y[2, 3]) and not y[2, :3].any()
     R.check(y[3:], R.norm(x[3:], None, 1e-6), "subnormal")
+    # gradients of rows so small that 1 / rms^3 is past fp32's range
+    x, g, w = _rnd(3, 72, seed=8, scale=1e-14), _rnd(3, 72, seed=9, scale=1e-3), _rnd(72, seed=10)
+    got, want = ops.block_norm_backward(g, x, w, 0.0), R.norm_backward(g, x, w, 0.0)
+    R.check(got[0], want[0], "grad_x of tiny rows")
+    R.check(got[1], want[1], "grad_weight of tiny rows")
     # a row's values never reach another row, whatever they are
     z = _rnd(4, 72, dtype=F16)
     z[2] = float("nan")
