@@ -294,7 +294,7 @@ def test_route_topk_records_its_gradient():
 
 # ---- norms ----
 
-WIDTHS = [33, 512, 520, 1024, 1031, 2048, 2056, 4096, 4104, 8192, 8200, 16392, 32768]
+WIDTHS = [33, 512, 520, 1024, 1031, 2048, 2056, 4096, 4099, 4104, 8192, 8200, 8203, 16392, 20001, 32768]
 TYPES = [(F16, F16), (BF16, BF16), (F32, F32), (F32, BF16), (BF16, F16), (F16, F32)]
 
 
@@ -332,7 +332,7 @@ def test_block_norm_of_short_rows(width):
 
 
 @pytest.mark.parametrize("tokens", [1, 2, 255, 257, 600, 1023, 2500])
-@pytest.mark.parametrize("width", [96, 2048])
+@pytest.mark.parametrize("width", [96, 515, 2048, 4100, 7168])
 def test_gradient_sums_over_many_tokens(tokens, width):
     """Every number of tokens a workgroup works off, the last of them short."""
     from mxmoe_amd import ops
