@@ -350,7 +350,7 @@ int mxmoe_route_topk_backward(const float* grad_weights, const void* router_logi
  * mxmoe_block_*_backward   the gradients of all inputs, sums over the tokens in fp32 and in a fixed order.  grad_y may be NULL (y was not used) and so may
  *     grad_h (grad_residual: what reaches x on other ways and is added to its gradient), not both.  grad_gate: gate_kind 1 packed [num_tokens] of gate_dtype,
  *     2 [num_tokens, K].  Gradients of the vectors that are given are written, in weight_dtype, also for no tokens (zeros).
- *     workspace: mxmoe_block_backward_workspace_bytes bytes, 16-byte aligned; NULL where no vector is given. */
+ *     workspace: mxmoe_block_backward_workspace_bytes bytes, 4-byte aligned; NULL where that is 0 or no vector is given. */
 int mxmoe_block_norm(const void* x, int64_t ldx, int x_dtype, const void* weight, int weight_dtype, float eps, int num_tokens, int K, void* y, int y_dtype, void* stream);
 int mxmoe_block_residual(const void* x, int64_t ldx, int x_dtype, const void* z, int64_t ldz, int z_dtype, int gate_kind, const void* gate, int64_t ld_gate, int gate_dtype, int sigmoid,
                          float factor, const void* scale, const void* norm_weight, const void* next_weight, int weight_dtype, float eps, int num_tokens, int K, void* h, void* y,

@@ -163,9 +163,9 @@ def test_block_norms_refuse(lib):
         assert norm(**bad) == 5, bad
     for bad in (dict(x=None), dict(z=None), dict(h=None), dict(kind=1)):
         assert res(**bad) == 5, bad
-    for bad in (dict(gh=None, gy=None), dict(x=None), dict(z=None), dict(gx=None), dict(gz=None), dict(g2=None), dict(ws=None), dict(kind=1, gate=p), dict(scale=p), dict(w1=p)):
+    for bad in (dict(gh=None, gy=None), dict(x=None), dict(z=None), dict(gx=None), dict(gz=None), dict(g2=None), dict(ws=None, t=5), dict(kind=1, gate=p), dict(scale=p), dict(w1=p)):
         assert bwd(**bad) == 5, bad
-    for bad in (dict(gy=None), dict(x=None), dict(gx=None), dict(gw=None), dict(ws=None)):
+    for bad in (dict(gy=None), dict(x=None), dict(gx=None), dict(gw=None), dict(ws=None, t=5)):
         assert nbwd(**bad) == 5, bad
     assert norm(t=0, x=None, y=None) == 0 and res(t=0, x=None, z=None, h=None) == 0
     assert lib.mxmoe_block_backward_workspace_bytes(0, 64) == 0 and lib.mxmoe_block_backward_workspace_bytes(7, 64) == 2 * 2 * 64 * 4
