@@ -173,6 +173,25 @@ def check_untracked_load_copies(asm: str) -> None:
                     work.append(n)
 
 
+def has_inline_assembly(src: Path, seen=None) -> bool:
+    """Whether a source or one of the project's headers that it includes has inline assembly (without any there are no hand-tracked loads to check)."""
+    seen = set() if seen is None else seen
+    src = src.resolve()
+    if src in seen:
+        return False
+    seen.add(src)
+    text = src.read_text()
+    if re.search(r"\basm\b", re.sub(r"//.*", "", text)):
+        return True
+    for name in re.findall(r'^\s*#include "([^"]+)"', text, re.M):
+        for base in (src.parent, CSRC / "include", PKG.parent / "include"):
+            if (base / name).exists():
+                if has_inline_assembly(base / name, seen):
+                    return True
+                break
+    return False
+
+
 def hipcc_build(sources, out: Path, extra=(), verbose: bool = False, jobs: int = 8) -> Path:
     """Compile each source to an object (in parallel) and link them into the shared library `out`."""
     from concurrent.futures import ThreadPoolExecutor
@@ -207,7 +226,7 @@ def hipcc_build(sources, out: Path, extra=(), verbose: bool = False, jobs: int =
 
     with ThreadPoolExecutor(max_workers=max(1, jobs)) as ex:
         jobs_ = [ex.submit(run, ["hipcc", *compile_flags, *extra, *inc, "-Rpass-analysis=kernel-resource-usage", "-c", str(s), "-o", str(o)]) for s, o in zip(sources, objs)]
-        jobs_ += [ex.submit(scan, s) for s in sources]
+        jobs_ += [ex.submit(scan, s) for s in sources if has_inline_assembly(s)]
         for j in jobs_:
             j.result()
     run(["hipcc", "--offload-arch=gfx950", "-shared", "-fPIC", *map(str, objs), "-o", str(out)])

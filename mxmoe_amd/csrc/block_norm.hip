@@ -4,11 +4,9 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
-#include <string>
-
 #include "../../include/mxmoe_amd.h"
 #include "include/mxmoe_block_norm.hpp"
-#include "include/mxmoe_launch.hpp"
+#include "include/mxmoe_error.hpp"
 
 namespace mxmoe {
 
@@ -115,25 +113,13 @@ static int run_block_norm_as(int xtype, int ztype, const BlockNormArgs& a, hipSt
   if (xtype == kF16) run_block_norm_z<_Float16, HAS_Z>(ztype, a, s);
   else if (xtype == kF32) run_block_norm_z<float, HAS_Z>(ztype, a, s);
   else run_block_norm_z<__bf16, HAS_Z>(ztype, a, s);
-  const hipError_t e = hipGetLastError();
-  if (e == hipSuccess) return 0;
-  last_error() = std::string("kernel launch failed: ") + hipGetErrorString(e);
-  return 4;
+  return launched();
 }
 
 int check_block_norm(const BlockNormArgs& a, int xtype, int ztype) {
-  if (a.T < 0 || a.K < 1 || a.K > kMaxNormRow || a.ldx < 0 || a.ldz < 0 || a.ldg < 0 || a.ldgh < 0 || a.ldgy < 0) {
-    last_error() = "block norms take rows of 1 .. 32768 elements, tokens and row strides >= 0";
-    return 3;
-  }
-  if (xtype < 0 || xtype > 2 || ztype < 0 || ztype > 2 || a.wtype < 0 || a.wtype > 2 || a.gate_type < 0 || a.gate_type > 2 || a.gate_kind < 0 || a.gate_kind > 2) {
-    last_error() = "float types are fp16 (0), fp32 (1) or bf16 (2), gates none (0), per token (1) or per element (2)";
-    return 3;
-  }
-  if (a.T && a.gate_kind && !a.gate) {
-    last_error() = "null pointer";
-    return 5;
-  }
+  if (a.T < 0 || a.K < 1 || a.K > kMaxNormRow || a.ldx < 0 || a.ldz < 0 || a.ldg < 0 || a.ldgh < 0 || a.ldgy < 0) return refuse(3, "block norms take rows of 1 .. 32768 elements, tokens and row strides >= 0");
+  if (xtype < 0 || xtype > 2 || ztype < 0 || ztype > 2 || a.wtype < 0 || a.wtype > 2 || a.gate_type < 0 || a.gate_type > 2 || a.gate_kind < 0 || a.gate_kind > 2) return refuse(3, "float types are fp16 (0), fp32 (1) or bf16 (2), gates none (0), per token (1) or per element (2)");
+  if (a.T && a.gate_kind && !a.gate) return refuse(5, "null pointer");
   return 0;
 }
 
@@ -155,10 +141,7 @@ int mxmoe_block_norm(const void* x, int64_t ldx, int x_dtype, const void* weight
   a.y = y;
   if (const int rc = check_block_norm(a, x_dtype, y_dtype)) return rc;
   if (num_tokens == 0) return 0;
-  if (!x || !y) {
-    last_error() = "null pointer";
-    return 5;
-  }
+  if (!x || !y) return refuse(5, "null pointer");
   return run_block_norm_as<false>(x_dtype, y_dtype, a, (hipStream_t)stream);
 }
 
@@ -186,15 +169,9 @@ int mxmoe_block_residual(const void* x, int64_t ldx, int x_dtype, const void* z,
   a.h = h;
   a.y = y;
   if (const int rc = check_block_norm(a, x_dtype, z_dtype)) return rc;
-  if (gate_kind == kElementGate && gate_dtype != z_dtype) {
-    last_error() = "a gate per element has the block output's type";
-    return 3;
-  }
+  if (gate_kind == kElementGate && gate_dtype != z_dtype) return refuse(3, "a gate per element has the block output's type");
   if (num_tokens == 0) return 0;
-  if (!x || !z || !h) {
-    last_error() = "null pointer";
-    return 5;
-  }
+  if (!x || !z || !h) return refuse(5, "null pointer");
   return run_block_norm_as<true>(x_dtype, z_dtype, a, (hipStream_t)stream);
 }
 

@@ -2,11 +2,9 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
-#include <string>
-
 #include "../../include/mxmoe_amd.h"
 #include "include/mxmoe_block_norm.hpp"
-#include "include/mxmoe_launch.hpp"
+#include "include/mxmoe_error.hpp"
 
 namespace mxmoe {
 
@@ -61,15 +59,9 @@ static int run_backward(int xtype, int ztype, bool has_z, BlockNormArgs& a, void
     const ColumnSumArgs c{a.partial, grid, planes, a.K, a.wtype, a.factor, a.scale, a.w1, grad_w2, grad_w1, grad_scale};
     hipLaunchKernelGGL(column_sum_kernel, dim3((a.K + 31) / 32, planes), dim3(1024), 0, s, c);
   }
-  const hipError_t e = hipGetLastError();
-  if (e == hipSuccess) return 0;
-  last_error() = std::string("kernel launch failed: ") + hipGetErrorString(e);
-  return 4;
+  return launched();
 }
-static int null_pointer() {
-  last_error() = "null pointer";
-  return 5;
-}
+static int null_pointer() { return refuse(5, "null pointer"); }
 
 }  // namespace mxmoe
 
@@ -136,18 +128,11 @@ int mxmoe_block_residual_backward(const void* grad_h, int64_t ld_grad_h, const v
   a.grad_gate = grad_gate;
   a.partial = reinterpret_cast<float*>(workspace);
   if (const int rc = check_block_norm(a, x_dtype, z_dtype)) return rc;
-  if (gate_kind == kElementGate && gate_dtype != z_dtype) {
-    last_error() = "a gate per element has the block output's type";
-    return 3;
-  }
+  if (gate_kind == kElementGate && gate_dtype != z_dtype) return refuse(3, "a gate per element has the block output's type");
   if ((scale && !grad_scale) || (norm_weight && !grad_norm_weight) || (next_weight && !grad_next_weight)) return null_pointer();
   if (num_tokens && (!x || !z || !grad_x || !grad_z || (gate_kind && !grad_gate) || ((scale || norm_weight || next_weight) && !workspace && mxmoe_block_backward_workspace_bytes(num_tokens, K)))) return null_pointer();
-  if (num_tokens && !grad_h && !grad_y) {
-    last_error() = "neither the gradient of h nor that of y is given";
-    return 5;
-  }
-  const int rc = run_backward(x_dtype, z_dtype, true, a, next_weight ? grad_next_weight : nullptr, norm_weight ? grad_norm_weight : nullptr, scale ? grad_scale : nullptr, (hipStream_t)stream);
-  return rc;
+  if (num_tokens && !grad_h && !grad_y) return refuse(5, "neither the gradient of h nor that of y is given");
+  return run_backward(x_dtype, z_dtype, true, a, next_weight ? grad_next_weight : nullptr, norm_weight ? grad_norm_weight : nullptr, scale ? grad_scale : nullptr, (hipStream_t)stream);
 }
 
 }  // extern "C"

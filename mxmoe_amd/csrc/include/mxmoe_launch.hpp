@@ -20,6 +20,7 @@
 #include <string>
 #include <vector>
 
+#include "mxmoe_error.hpp"
 #include "mxmoe_tiles.hpp"
 #include "mxmoe_grp_tiles.hpp"
 #include "mxmoe_few_tiles.hpp"
@@ -416,11 +417,6 @@ struct FusedKernel {
 inline std::vector<FusedKernel>& registry() {
   static std::vector<FusedKernel> r;
   return r;
-}
-
-inline std::string& last_error() {
-  static thread_local std::string e;
-  return e;
 }
 
 template <int WBITS, int BM, int BN>

@@ -15,10 +15,9 @@
 #include <stdint.h>
 
 #include <algorithm>
-#include <string>
 
 #include "../../include/mxmoe_amd.h"
-#include "include/mxmoe_launch.hpp"
+#include "include/mxmoe_error.hpp"
 #include "include/mxmoe_perm.hpp"
 #include "include/mxmoe_rows.hpp"
 #include "include/mxmoe_vec8.hpp"
@@ -423,16 +422,6 @@ __global__ void __launch_bounds__(256) route_backward_kernel(const RouteGradArgs
   }
 }
 
-static int refuse(int code, const char* what) {
-  last_error() = what;
-  return code;
-}
-static int launched() {
-  const hipError_t e = hipGetLastError();
-  if (e == hipSuccess) return 0;
-  last_error() = std::string("kernel launch failed: ") + hipGetErrorString(e);
-  return 4;
-}
 static int permute_stride(long slots) { return ((int)((slots + kCountChunk - 1) / kCountChunk) + 3) & ~3; }
 
 template <typename ID>

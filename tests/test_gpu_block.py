@@ -637,6 +637,30 @@ def test_operators_in_graphs_and_on_another_stream():
     assert all(torch.equal(a, b) for a, b in zip(again, wants[1]))
 
 
+def test_two_threads_on_two_streams():
+    import threading
+
+    states, wants, gots = [_state(5), _state(6)], [], [None, None]
+    for s in states:
+        wants.append([o.clone() for o in _all_operators(s)])
+    torch.cuda.synchronize()
+
+    def work(i):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            for _ in range(20):
+                gots[i] = _all_operators(states[i])
+        stream.synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for got, want in zip(gots, wants):
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 def test_a_recorded_call_under_capture_is_refused():
     from mxmoe_amd import ops
 
