@@ -45,7 +45,7 @@ struct BlockNormArgs {
 
 // sigmoid(g) = 1 / (1 + exp(-g)) and its slope a (1 - a), both from e = exp(-|g|), which neither overflows nor lets 1 - a cancel: a = 1 / (1 + e) for g >= 0 and e / (1 + e)
 // below, slope = e / (1 + e)^2.  The exponential is 2^(x log2 e) with the product's rounding error put back to first order, the quotient the reciprocal
-// instruction's (one unit in the last place): 14 instructions for both, where expf and a division for each took some 45 and were half of the backward kernel's time.
+// instruction's (one unit in the last place): 14 instructions for both, where expf and a division for each took some 45 and were a third of the backward kernel's time.
 struct Sigmoid {
   float a, slope;
   __device__ __forceinline__ explicit Sigmoid(float g) {
