@@ -78,6 +78,24 @@ def _output(out, like: torch.Tensor, rows: int, k: int, dtype) -> torch.Tensor:
     return out
 
 
+def _span(x: torch.Tensor):
+    """First byte of x's elements and the one behind the last."""
+    first = x.data_ptr()
+    return first, first + (sum((n - 1) * st for n, st in zip(x.shape, x.stride())) + 1) * x.element_size() if x.numel() else first
+
+
+def _apart(out: torch.Tensor, *inputs, same=()) -> None:
+    """Refuse an `out` that shares memory with an input: rows of it would be overwritten before others have read them.  With those in `same` it may be one and the same tensor
+    (each thread reads its elements of a row before it writes them)."""
+    first, end = _span(out)
+    for x in (*inputs, *same):
+        if x is None:
+            continue
+        a, b = _span(x)
+        if a < end and first < b and not (any(x is y for y in same) and a == first and x.dtype == out.dtype and x.shape == out.shape and x.stride() == out.stride()):
+            raise ValueError("out shares memory with an input")
+
+
 def _recorded(*tensors, out=None) -> bool:
     """Whether autograd is to record a call with these inputs."""
     if not torch.is_grad_enabled():
@@ -123,6 +141,8 @@ def _permute(hidden, topk_ids, num_experts, out, perm):
     ids = topk_ids.contiguous()
     topk, wide, dev = ids.shape[1], ids.dtype is torch.int64, x.device
     rows = _output(out, x, t * topk, k, x.dtype)
+    if out is not None:
+        _apart(out, x, ids)
     row_of_slot = torch.empty((t, topk), dtype=torch.int32, device=dev) if wide else torch.empty_like(ids)
     recv = torch.empty(max(num_experts, 0), dtype=torch.int64, device=dev)
     need = _lib.load().mxmoe_permute_tokens_workspace_bytes(t, topk, num_experts) if t * topk > 4096 else 0
@@ -183,6 +203,8 @@ def _unpermute(rows, row_of_slot, topk_weights, shared, out):
     w = None if topk_weights is None else _weights(topk_weights, m, index)
     sh = None if shared is None else _rows(shared, "shared", (t, k), x.dtype, index)
     y = _output(out, x if sh is None else sh, t, k, x.dtype)
+    if out is not None:
+        _apart(out, x, m, w, same=(sh,))
     _call(index, "mxmoe_unpermute_tokens", x.data_ptr(), x.stride(0), n, m.data_ptr(), None if w is None else w.data_ptr(), None if sh is None else sh.data_ptr(),
           0 if sh is None else sh.stride(0), _TYPES[x.dtype], t, topk, k, y.data_ptr())
     return y
@@ -217,6 +239,8 @@ def unpermute_tokens_backward(grad_out: torch.Tensor, rows: torch.Tensor | None,
         grad_rows = torch.zeros((num_rows, k), dtype=g.dtype, device=g.device)
     else:
         grad_rows = _output(out, g if x is None else x, num_rows, k, g.dtype)
+    if out is not None:
+        _apart(out, g, m, w, same=(x,))
     grad_w = None if w is None or x is None else torch.empty_like(w)
     _call(index, "mxmoe_unpermute_tokens_backward", g.data_ptr(), g.stride(0), None if x is None else x.data_ptr(), 0 if x is None else x.stride(0), num_rows, m.data_ptr(),
           None if w is None else w.data_ptr(), _TYPES[g.dtype], t, topk, k, grad_rows.data_ptr(), out is not None, None if grad_w is None else grad_w.data_ptr())
@@ -276,6 +300,8 @@ def _norm(x, weight, eps, out_dtype, out):
     elif out_dtype not in _TYPES:
         raise ValueError(_NO_TYPE.format("output", out_dtype))
     y = _output(out, xr, t, k, out_dtype)
+    if out is not None:
+        _apart(out, w, same=(xr,))
     _call(index, "mxmoe_block_norm", xr.data_ptr(), xr.stride(0), xt, None if w is None else w.data_ptr(), 1 if w is None else _TYPES[w.dtype], eps, t, k, y.data_ptr(), _TYPES[out_dtype])
     return y
 
@@ -355,7 +381,7 @@ def block_residual(x: torch.Tensor, z: torch.Tensor, *, gate: torch.Tensor | Non
 
     norm(z) = z / sqrt(mean(z^2) + eps) * norm_weight, or z itself without `norm_weight`.  `gate` per token ([T] or [T, 1]) or per element ([T, K], z's dtype), through a
     sigmoid with gate_act="sigmoid" (a shared expert's gate, say).  `scale`: a number, or one per channel [K].  The vectors have one dtype.  Everything is fp32 inside; y
-    is computed from h before its rounding.  `out` (x itself is allowed) receives h."""
+    is computed from h before its rounding.  `out` (x or z itself is allowed) receives h."""
     if out is None:
         got = (_fast or _calls()).block_residual(x, z, gate, gate_act, scale, norm_weight, next_weight, eps)
         if got is not None:
@@ -373,6 +399,8 @@ def _residual(x, z, gate, gate_act, scale, norm_weight, next_weight, eps, out):
     if out is not None and xr is not x and out.data_ptr() == x.data_ptr():
         raise ValueError("out may be x only where x's elements lie side by side")
     h = _output(out, xr, t, k, xr.dtype)
+    if out is not None:
+        _apart(out, vec, w1, w2, *(() if g is None or g.dim() == 2 and g.shape[1] == k else (g,)), same=(xr, zr, g if g is not None and g.dim() == 2 and g.shape[1] == k else None))
     y = None if w2 is None else _output(None, zr, t, k, zr.dtype)
     _call(xr.get_device(), "mxmoe_block_residual", *args, eps, t, k, h.data_ptr(), None if y is None else y.data_ptr())
     return h if y is None else (h, y)

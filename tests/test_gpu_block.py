@@ -278,6 +278,70 @@ def test_route_topk_backward(t, e, k, dtype, renormalise):
     assert not got[-1].any()
 
 
+@pytest.mark.parametrize("masked", [float("-inf"), torch.finfo(F16).min])
+@pytest.mark.parametrize("renormalise", [False, True])
+def test_route_topk_backward_of_masked_experts(masked, renormalise):
+    """Experts switched off by their logit: no gradient of their own, and that of the others as if they were not there."""
+    from mxmoe_amd import ops
+
+    logits, dw = _rnd(40, 24, dtype=F16, seed=1), _rnd(40, 3, seed=2)
+    live = torch.arange(0, 24, 3, device=DEV)                                                  # (8 experts)
+    few = logits[:, live].contiguous()
+    full = torch.full_like(logits, masked).index_copy(1, live, few)
+    ids = ops.route_topk(few, 3, renormalise)[0]
+    want = R.route_backward(dw, few, ids, renormalise)
+    got = ops.route_topk_backward(dw, full, live[ids.long()], renormalise)
+    R.check(got[:, live], want, "grad of the live experts")
+    rest = torch.ones(24, dtype=torch.bool, device=DEV).index_fill(0, live, False)
+    assert not got[:, rest].any()
+    # a masked expert among the chosen ones has probability 0
+    ids = live[ids.long()]
+    ids[:, 2] = 1
+    got = ops.route_topk_backward(dw, full, ids, renormalise)
+    assert torch.isfinite(got).all() and not got[:, rest].any() and got[:, live].abs().sum() > 0
+
+
+def test_what_stands_in_masked_places_is_not_read():
+    from mxmoe_amd import ops
+
+    x, g = _rnd(6, 72, dtype=BF16, seed=1), _rnd(6, 72, dtype=BF16, seed=2)
+    ids = _ids(6, 2, 4, 3)
+    ids[[1, 4]] = -1                                                                           # (padding tokens)
+    x[[1, 4]], g[[1, 4]] = float("nan"), float("inf")
+    rows, m, recv = ops.permute_tokens(x, ids, 4)
+    assert torch.isfinite(rows).all() and not rows[8:].any()
+    w = _rnd(6, 2, seed=4)
+    w[[1, 4]] = float("nan")
+    out = ops.unpermute_tokens(rows, m, w)
+    assert torch.isfinite(out).all() and not out[[1, 4]].any()
+    gr, gw = ops.unpermute_tokens_backward(g, rows, m, w)
+    assert torch.isfinite(gr).all() and not gr[8:].any() and torch.isfinite(gw).all() and not gw[[1, 4]].any()
+
+
+def test_outputs_that_share_memory_with_inputs():
+    from mxmoe_amd import ops
+
+    x, ids = _rnd(6, 64, dtype=F16, seed=1), torch.tensor([[2], [0], [1], [0], [2], [1]], dtype=torch.int32, device=DEV)
+    rows, m, _ = ops.permute_tokens(x, ids, 3)
+    buf = torch.zeros(7, 64, dtype=F16, device=DEV)
+    bad = [lambda: ops.permute_tokens(x, ids, 3, out=x), lambda: ops.unpermute_tokens(rows, m, out=rows), lambda: ops.unpermute_tokens_backward(x, None, m, out=x),
+           lambda: ops.block_norm(buf[:6], out=buf[1:]), lambda: ops.block_residual(buf[:6], x, out=buf[1:]), lambda: ops.block_residual(x, buf[:6], out=buf[1:]),
+           lambda: ops.unpermute_tokens(rows, m, shared=buf[:6], out=buf[1:])]
+    for call in bad:
+        with pytest.raises(ValueError, match="shares memory"):
+            call()
+    # the same tensor where a row's elements are read before they are written
+    for width in (64, 61, 515, 2055):
+        x, z, gate, w, r, sh = (_rnd(6, width, dtype=F16, seed=i) for i in range(6))
+        tw = _rnd(6, 1, seed=7)
+        calls = [(x, lambda t, o: ops.block_norm(t, out=o)), (x, lambda t, o: ops.block_residual(t, z, gate=gate, norm_weight=w[0], out=o)),
+                 (z, lambda t, o: ops.block_residual(x, t, gate=gate, norm_weight=w[0], out=o)), (gate, lambda t, o: ops.block_residual(x, z, gate=t, norm_weight=w[0], out=o)),
+                 (sh, lambda t, o: ops.unpermute_tokens(r, m, shared=t, out=o)), (r, lambda t, o: ops.unpermute_tokens_backward(x, t, m, tw, out=o)[0])]
+        for tensor, call in calls:
+            want, mine = call(tensor, None), tensor.clone()
+            assert call(mine, mine) is mine and torch.equal(mine, want)
+
+
 def test_route_topk_records_its_gradient():
     from mxmoe_amd import ops
 
@@ -577,6 +641,31 @@ def test_calls_in_python_and_in_the_extension_are_the_same(monkeypatch):
     for c, b in zip((2.0, 2, None), scaled):
         assert torch.equal(ops.block_residual(s["x"], s["x"], scale=c), b)
         assert torch.equal(ops.block_residual(s["x"].clone().requires_grad_(), s["x"], scale=c).detach(), b)
+
+
+def test_calls_with_another_device_current(monkeypatch):
+    """What a call does whose tensors are not on the current device (here: a current device that claims to be another)."""
+    from mxmoe_amd import _lib as L
+    from mxmoe_amd import block
+
+    s = _state(4)
+    want = _all_operators(s)
+    raw = torch._C._cuda_getCurrentRawStream
+    block._fast.bind(*block_addresses(), lambda: 7, raw)                                       # the extension leaves such calls to Python
+    monkeypatch.setattr(L, "current_device", lambda: 7)
+    try:
+        got = _all_operators(s)
+    finally:
+        block._fast.bind(*block_addresses(), torch._C._cuda_getDevice, raw)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def block_addresses():
+    import ctypes as C
+
+    from mxmoe_amd import _lib as L
+
+    return [C.cast(getattr(L.load(), name), C.c_void_p).value for name in L._CALLS]
 
 
 # ---- streams, graphs, refusals ----
