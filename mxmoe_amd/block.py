@@ -214,9 +214,8 @@ def unpermute_tokens_backward(grad_out: torch.Tensor, rows: torch.Tensor | None,
                               num_rows: int | None = None, out: torch.Tensor | None = None):
     """Gradients of `unpermute_tokens` -> (grad_rows [rows, K], grad_weights fp32 [T, k]); that of `shared` is grad_out itself.
 
-    grad_rows[row_of_slot[t, s]] = w[t, s] * grad_out[t]; rows that belong to dropped slots (those behind the last routed one, as `permute_tokens` numbers them) are zero,
-    with `out` left as they were.  The map names every row once, as `permute_tokens` writes it; one of `build_permutation` (-1 for dropped slots, whose rows it does not
-    name) goes with the routed rows alone, `rows[:routed]`.  `rows` None (then `num_rows`, default T * k, says how many there are), or no weights: grad_weights is None."""
+    grad_rows[row_of_slot[t, s]] = w[t, s] * grad_out[t].  The map names a row at most once and leaves no gaps, as `permute_tokens` and `build_permutation` write it; the rows
+    behind the named ones, those of dropped slots among them, are zero, with `out` left as they were.  `rows` None (then `num_rows`, default T * k, says how many there are), or no weights: grad_weights is None."""
     if out is None:
         got = (_fast or _calls()).unpermute_tokens_backward(grad_out, rows, row_of_slot, topk_weights)
         if got is not None:
@@ -235,10 +234,7 @@ def unpermute_tokens_backward(grad_out: torch.Tensor, rows: torch.Tensor | None,
         num_rows = x.shape[0]
     elif num_rows is None:
         num_rows = t * topk
-    if num_rows > t * topk and out is None:  # rows that no slot can name
-        grad_rows = torch.zeros((num_rows, k), dtype=g.dtype, device=g.device)
-    else:
-        grad_rows = _output(out, g if x is None else x, num_rows, k, g.dtype)
+    grad_rows = _output(out, g if x is None else x, num_rows, k, g.dtype)
     if out is not None:
         _apart(out, g, m, w, same=(x,))
     grad_w = None if w is None or x is None else torch.empty_like(w)

@@ -170,7 +170,7 @@ PyObject* unpermute_tokens_backward(PyObject*, PyObject* const* args, Py_ssize_t
   if (!ok || !g.defined() || !x.defined() || !w.defined() || !x.is_cuda()) NOT_MINE;
   const int device = current_device();
   if (!rows(g, device) || !rows(x, device) || x.size(1) != g.size(1) || x.scalar_type() != g.scalar_type() || !slot_map(m, device) || m.size(0) != g.size(0) || !weights_of(w, m, device) ||
-      x.size(0) > m.numel() || x.size(1) > kMost)
+      x.size(0) > kMost || x.size(1) > kMost)
     NOT_MINE;
   at::Tensor grad_rows = rows_like(x, x.size(0), x.size(1), x.scalar_type()), grad_weights = rows_like(w, m.size(0), m.size(1), at::kFloat);
   if (lib.unpermute_backward(ptr(g), g.stride(0), ptr(x), x.stride(0), (int)x.size(0), (const int32_t*)ptr(m), (const float*)ptr(w), float_type(x), (int)m.size(0), (int)m.size(1), (int)x.size(1),

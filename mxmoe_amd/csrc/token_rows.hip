@@ -286,6 +286,12 @@ __global__ void __launch_bounds__(256) unpermute_kernel(const GatherArgs a) {
 //
 // One workgroup of NT threads a token; S slots at a time (of a top-k of 2, 4 or more).  grad_out's piece stays in registers while it is multiplied with each slot's row (the
 // weight's gradient) and by each weight (the row's gradient): one pass over everything.
+//
+// Rows that nobody owns get zeros: those of dropped slots from the slot's workgroup, whose entry says which row it is (-2 - row); the rest, which a map of -1 entries or a buffer with
+// more rows than slots leaves, from `fillers` workgroups in front of the others, which count the entries that name a row.  Those rows are the last ones, because the sort leaves
+// no gaps.  (The count is four bytes a slot for each of them, beside the slot's two rows.)
+constexpr int kFillers = 16;
+typedef int Slots4 __attribute__((ext_vector_type(4), aligned(4)));
 struct UngatherArgs {
   const void* grad_out;
   long ld_grad;
@@ -294,16 +300,36 @@ struct UngatherArgs {
   int num_rows;
   const int32_t* row_of_slot;
   const float* weights;
-  int T, topk, K, keep_tail;
+  int T, topk, K, keep_tail, fillers;
   void* grad_rows;
   float* grad_weights;    // or null
 };
 template <typename T, int NT, int S>
 __global__ void __launch_bounds__(NT) unpermute_backward_kernel(const UngatherArgs a) {
   __shared__ float sums[2][S * (NT / 64)];
-  const long t = folded_block();
+  const long t = folded_block() - a.fillers;
   const int C = (a.K + 7) >> 3;
   if (t >= a.T) return;
+  if (t < 0) {
+    __shared__ int named[NT / 64];
+    auto names = [&](int r) { return (r >= 0 && r < a.num_rows) || (r <= -2 && -2 - r < a.num_rows); };
+    int n = 0;
+    const long slots = (long)a.T * a.topk, quads = slots >> 2;
+#pragma unroll 8
+    for (long q = threadIdx.x; q < quads; q += NT) {
+      const Slots4 r = reinterpret_cast<const Slots4*>(a.row_of_slot)[q];
+      n += names(r[0]) + names(r[1]) + names(r[2]) + names(r[3]);
+    }
+    if (4 * quads + threadIdx.x < slots) n += names(a.row_of_slot[4 * quads + threadIdx.x]);
+    n = wave_last(wave_inclusive_scan(n));
+    if ((threadIdx.x & 63) == 0) named[threadIdx.x >> 6] = n;
+    __syncthreads();
+    n = 0;
+    for (int w = 0; w < NT / 64; ++w) n += named[w];
+    for (long row = n + t + a.fillers; row < a.num_rows; row += a.fillers)
+      for (int c = threadIdx.x; c < C; c += NT) store_piece(reinterpret_cast<T*>(a.grad_rows) + row * a.K, c, a.K, typename Piece<T>::raw{});
+    return;
+  }
   const T* g_row = reinterpret_cast<const T*>(a.grad_out) + t * a.ld_grad;
   for (int s0 = 0, turn = 0; s0 < a.topk; s0 += S, turn ^= 1) {
     int r[S];
@@ -455,9 +481,9 @@ static void run_unpermute(const GatherArgs& a, hipStream_t s) {
 }
 template <typename T, int NT>
 static void run_unpermute_backward_as(const UngatherArgs& a, hipStream_t s) {
-  if (a.topk <= 2) hipLaunchKernelGGL((unpermute_backward_kernel<T, NT, 2>), folded_grid(a.T), dim3(NT), 0, s, a);
-  else if (a.topk <= 4) hipLaunchKernelGGL((unpermute_backward_kernel<T, NT, 4>), folded_grid(a.T), dim3(NT), 0, s, a);
-  else hipLaunchKernelGGL((unpermute_backward_kernel<T, NT, 8>), folded_grid(a.T), dim3(NT), 0, s, a);
+  if (a.topk <= 2) hipLaunchKernelGGL((unpermute_backward_kernel<T, NT, 2>), folded_grid((long)a.T + a.fillers), dim3(NT), 0, s, a);
+  else if (a.topk <= 4) hipLaunchKernelGGL((unpermute_backward_kernel<T, NT, 4>), folded_grid((long)a.T + a.fillers), dim3(NT), 0, s, a);
+  else hipLaunchKernelGGL((unpermute_backward_kernel<T, NT, 8>), folded_grid((long)a.T + a.fillers), dim3(NT), 0, s, a);
 }
 template <typename T>
 static void run_unpermute_backward(const UngatherArgs& a, hipStream_t s) {
@@ -532,9 +558,10 @@ int mxmoe_unpermute_tokens_backward(const void* grad_out, int64_t ld_grad, const
                                     int num_tokens, int topk, int K, void* grad_rows, int keep_tail, float* grad_weights, void* stream) {
   if (!token_sizes_ok(num_tokens, topk, 1, K) || num_rows < 0) return refuse(3, kTokenSizes);
   if (dtype < 0 || dtype > 2 || ld < 0 || ld_grad < 0) return refuse(3, "rows as fp16 (0), fp32 (1) or bf16 (2), row strides >= 0");
-  if (num_tokens == 0) return 0;
-  if (!grad_out || !row_of_slot || (num_rows && !grad_rows) || (grad_weights && num_rows && !rows)) return refuse(5, "null pointer");
-  const UngatherArgs a{grad_out, (long)ld_grad, rows, (long)ld, num_rows, row_of_slot, topk_weights, num_tokens, topk, K, keep_tail != 0, grad_rows, grad_weights};
+  const int fillers = num_rows && !keep_tail ? kFillers : 0;
+  if (num_tokens + fillers == 0) return 0;
+  if ((num_rows && !grad_rows) || (num_tokens && (!grad_out || !row_of_slot || (grad_weights && num_rows && !rows)))) return refuse(5, "null pointer");
+  const UngatherArgs a{grad_out, (long)ld_grad, rows, (long)ld, num_rows, row_of_slot, topk_weights, num_tokens, topk, K, keep_tail != 0, fillers, grad_rows, grad_weights};
   hipStream_t s = (hipStream_t)stream;
   if (dtype == kF16) run_unpermute_backward<_Float16>(a, s);
   else if (dtype == kF32) run_unpermute_backward<float>(a, s);

@@ -123,7 +123,7 @@ def test_unpermute_tokens_refuses(lib):
         assert fwd(**bad) == 5, bad
     for bad in (dict(g=None), dict(m=None), dict(gr=None), dict(rows=None)):
         assert bwd(**bad) == 5, bad
-    assert fwd(t=0, rows=None, m=None, out=None) == 0 and bwd(t=0, g=None, m=None, gr=None) == 0
+    assert fwd(t=0, rows=None, m=None, out=None) == 0 and bwd(t=0, n=0, g=None, m=None, gr=None) == 0 and bwd(t=0, gr=None) == 5
 
 
 def test_route_topk_backward_refuses(lib):

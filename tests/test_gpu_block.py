@@ -148,7 +148,11 @@ def test_unpermute_tokens_maps_of_the_other_permutation_and_bad_ones():
     assert torch.equal(ops.unpermute_tokens(y, other, w), ops.unpermute_tokens(y, m, w))
     routed = int((m >= 0).sum())
     a, b = ops.unpermute_tokens_backward(g, y, other, w), ops.unpermute_tokens_backward(g, y, m, w)
-    assert torch.equal(a[0][:routed], b[0][:routed]) and torch.equal(a[1], b[1])
+    assert torch.equal(a[0], b[0]) and not a[0][routed:].any() and torch.equal(a[1], b[1])
+    assert torch.equal(ops.unpermute_tokens_backward(g, y[:routed], other, w)[0], b[0][:routed])
+    leaf = y.clone().requires_grad_()
+    ops.unpermute_tokens(leaf, other, w).backward(g)
+    assert torch.equal(leaf.grad, b[0])
     more = torch.cat([y, y[:5]])                                                               # (rows that no slot can name)
     c = ops.unpermute_tokens_backward(g, more, m, w)
     assert torch.equal(c[0][:60], b[0]) and not c[0][60:].any() and torch.equal(c[1], b[1])
@@ -163,6 +167,13 @@ def test_unpermute_tokens_maps_of_the_other_permutation_and_bad_ones():
     assert not ops.unpermute_tokens(y, torch.full((4, 2), -1, dtype=torch.int32, device=DEV)).any()
     assert not ops.unpermute_tokens(y[:0], torch.full((4, 2), -1, dtype=torch.int32, device=DEV)).any()
     assert ops.unpermute_tokens(y, m[:0]).shape == (0, 64) and ops.unpermute_tokens_backward(g[:0], y[:0], m[:0], w[:0])[0].shape == (0, 64)
+    nothing = ops.unpermute_tokens_backward(g[:0], y, m[:0], w[:0])
+    assert nothing[0].shape == (60, 64) and not nothing[0].any() and nothing[1].shape == (0, 3)
+    # many dropped slots of -1
+    ids = _ids(3000, 4, 9, 5, 0.9)
+    g, w = _rnd(3000, 40, dtype=F16, seed=6), _rnd(3000, 4, seed=7)
+    m, other = ops.permute_tokens(g, ids, 9)[1], ops.build_permutation(ids, 9, with_inverse=True)[4].view(3000, 4)
+    assert torch.equal(ops.unpermute_tokens_backward(g, None, other, w)[0], ops.unpermute_tokens_backward(g, None, m, w)[0])
 
 
 def test_infinities_stay_in_their_rows():
